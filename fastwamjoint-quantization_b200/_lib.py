@@ -6,7 +6,7 @@ present when a kernel is requested, the call raises.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 from functools import lru_cache
 from pathlib import Path
 
@@ -23,7 +23,38 @@ WEIGHTS_PREPACKED = 4  # OR-ed onto the weight-scale mode: weights are int8 [N, 
 CODES_INT4_RANGE = 2  # OR-ed onto the layout for sq_gemm: every code lies in [-8, 7]
 WSCALE_CHANNEL_F32, WSCALE_GROUP_F16 = 0, 1
 NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2
+ROTARY_AXES = 4
+ROTARY_INTERLEAVED, ROTARY_HALF = 0, 1
+ROTARY_NORM_NONE, ROTARY_NORM_HEAD, ROTARY_NORM_TOKEN = 0, 1, 2
+POS_INT32, POS_INT64, POS_FP32 = 0, 1, 2
 ACT_FN_NONE, ACT_FN_GELU = 0, 1
+
+
+class Param(ctypes.Structure):
+    """``SqParam``: rows of parameters."""
+    _fields_ = [("data", c_void_p), ("row_stride", c_int64), ("span", c_int64), ("is_fp32", c_int32), ("reserved", c_int32)]
+
+
+class BlockNorm(ctypes.Structure):
+    """``SqBlockNorm``."""
+    _fields_ = [("x", c_void_p), ("branch", c_void_p),
+                *((name, Param) for name in ("gate", "post_weight", "post_bias", "weight", "bias", "mod_scale", "mod_shift")),
+                ("h_out", c_void_p), ("z_out", c_void_p), ("scales", c_void_p), ("scales_row_stride", c_int64),
+                ("scales_group_stride", c_int64), ("rows", c_int64), ("width", c_int64), ("residual_scale", c_float),
+                ("eps", c_float), ("dtype", c_int32), ("post_kind", c_int32), ("norm_kind", c_int32), ("reserved", c_int32)]
+
+
+class Rotary(ctypes.Structure):
+    """``SqRotary``."""
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("q_out", c_void_p), ("k_out", c_void_p),
+                *((name, c_int64 * 3) for name in ("q_strides", "k_strides", "q_out_strides", "k_out_strides")),
+                ("q_weight", c_void_p), ("k_weight", c_void_p), ("positions", c_void_p),
+                ("position_batch_stride", c_int64), ("position_token_stride", c_int64), ("inv_freq", c_void_p),
+                ("batch", c_int64), ("length", c_int64), ("heads", c_int32), ("kv_heads", c_int32), ("dim", c_int32),
+                ("axes", c_int32), ("sections", c_int32 * ROTARY_AXES), ("dtype", c_int32), ("layout", c_int32),
+                ("norm", c_int32), ("position_type", c_int32), ("q_weight_fp32", c_int32), ("k_weight_fp32", c_int32),
+                ("eps", c_float), ("reserved", c_int32)]
+
 
 _SIGNATURES = {
     "sq_prepass": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p, c_int,
@@ -66,6 +97,14 @@ _SIGNATURES = {
     "sq_linear_noalloc": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p, c_int,
                                   c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64,
                                   c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
+    "sq_fp8_quantize": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int64, c_void_p]),
+    "sq_fp8_gemm": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                            c_int64, c_int64, c_int64, c_void_p]),
+    "sq_fp8_linear": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                              c_void_p, c_size_t, c_void_p]),
+    "sq_fp8_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "sq_block_norm": (c_int, [c_void_p, c_void_p]),
+    "sq_rotary": (c_int, [c_void_p, c_void_p]),
     "sq_wait_probe": (c_int, [c_int64, c_void_p, c_void_p]),
     "sq_device_status": (c_int, []),
     "sq_status_string": (c_char_p, [c_int]),

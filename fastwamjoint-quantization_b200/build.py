@@ -19,8 +19,9 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 LIB = HERE / "lib" / "libsq_b200.so"
-SOURCES = ("sq_prepass.cu", "sq_gemm_tc.cu", "sq_gemm_ts.cu", "sq_api.cu")
-HEADERS = ("sq_internal.h", "sq_ptx.cuh", "../../include/sq_b200.h")
+SOURCES = ("sq_prepass.cu", "sq_gemm_tc.cu", "sq_gemm_ts.cu", "sq_fp8_gemm.cu", "sq_block_norm.cu", "sq_rotary.cu",
+           "sq_api.cu")
+HEADERS = ("sq_internal.h", "sq_ptx.cuh", "sq_rows.cuh", "../../include/sq_b200.h")
 NVCC_FLAGS = ("-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden")
 

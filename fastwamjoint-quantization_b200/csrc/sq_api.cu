@@ -325,6 +325,50 @@ int sq_wait_probe(int64_t limit_us, long long* waited_ns, void* stream) {
   return sq::launch_wait_probe(limit_us, waited_ns, static_cast<cudaStream_t>(stream));
 }
 
+int sq_fp8_quantize(const void* x, int x_dtype, int64_t rows, int64_t K, int input_activation, void* codes, float* scales,
+                    int64_t scales_row_stride, int64_t scales_group_stride, void* stream) {
+  return sq::launch_fp8_quantize(x, x_dtype, rows, K, input_activation, codes, scales, scales_row_stride, scales_group_stride,
+                                 static_cast<cudaStream_t>(stream));
+}
+
+int sq_fp8_gemm(const void* codes, const float* scales, int64_t scales_row_stride, int64_t scales_group_stride,
+                const void* weight, const float* weight_scales, const void* bias, void* out, int out_dtype, int64_t M,
+                int64_t N, int64_t K, void* stream) {
+  return sq::launch_fp8_gemm({codes, scales, scales_row_stride, scales_group_stride, weight, weight_scales, bias, out, out_dtype,
+                              M, N, K},
+                             static_cast<cudaStream_t>(stream));
+}
+
+size_t sq_fp8_workspace_bytes(int64_t rows, int64_t K) {
+  if (rows < 0 || K < 0) return 0;
+  return sq::round256(static_cast<size_t>(rows) * static_cast<size_t>(K)) +
+         sq::round256(static_cast<size_t>(rows) * static_cast<size_t>((K + 127) / 128) * 4u);
+}
+
+int sq_fp8_linear(const void* x, int x_dtype, int64_t rows, int64_t K, int64_t N, int input_activation, const void* weight,
+                  const float* weight_scales, const void* bias, void* out, void* workspace, size_t workspace_bytes,
+                  void* stream) {
+  if (workspace == nullptr && rows > 0) return SQ_ERR_NULL;
+  if (workspace_bytes < sq_fp8_workspace_bytes(rows, K)) return SQ_ERR_WORKSPACE;
+  // codes, then the scales with a run's tokens next to each other: what a warp of the product reads together
+  float* scales = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
+                                           sq::round256(static_cast<size_t>(rows) * static_cast<size_t>(K)));
+  sq::Fp8GemmArgs gemm = {workspace, scales, 1, rows, weight, weight_scales, bias, out, x_dtype, rows, N, K, true};
+  const int refused = sq::validate_fp8_gemm(gemm);  // before the quantizer: a refused call launches nothing
+  if (refused != SQ_OK || rows == 0) return refused;
+  const int status = sq::launch_fp8_quantize(x, x_dtype, rows, K, input_activation, workspace, scales, 1, rows,
+                                             static_cast<cudaStream_t>(stream));
+  return status != SQ_OK ? status : sq::launch_fp8_gemm(gemm, static_cast<cudaStream_t>(stream));
+}
+
+int sq_block_norm(const SqBlockNorm* args_host, void* stream) {
+  return args_host == nullptr ? SQ_ERR_NULL : sq::launch_block_norm(*args_host, static_cast<cudaStream_t>(stream));
+}
+
+int sq_rotary(const SqRotary* args_host, void* stream) {
+  return args_host == nullptr ? SQ_ERR_NULL : sq::launch_rotary(*args_host, static_cast<cudaStream_t>(stream));
+}
+
 size_t sq_workspace_bytes(int64_t M, int64_t K) {
   if (M < 0 || K < 0) return 0;
   return sq::round256(static_cast<size_t>(M) * static_cast<size_t>(K)) + sq::round256(static_cast<size_t>(M) * 4u);
@@ -526,6 +570,10 @@ const char* sq_status_string(int status) {
     case 9107: return "device: TMA producer timed out waiting for a free row-scale slot";
     case 9108: return "device: drain warps timed out meeting around a split tile";
     case 9109: return "device: drain warp timed out waiting for row scales";
+    case 9201: return "device: e4m3 product, TMA producer timed out waiting for a free stage";
+    case 9202: return "device: e4m3 product, MMA warp timed out waiting for a free accumulator";
+    case 9203: return "device: e4m3 product, MMA warp timed out waiting for operands";
+    case 9204: return "device: e4m3 product, drain warp timed out waiting for an accumulator";
     case 9190: return "device: the wait probe gave up, as it is meant to";
     case 9001: return "device: TMA producer timed out waiting for a free stage";
     case 9002: return "device: MMA warp timed out waiting for a free accumulator";

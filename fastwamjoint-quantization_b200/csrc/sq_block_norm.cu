@@ -1,0 +1,377 @@
+// Norms before and after a block with its gate and residual scale, and the e4m3 quantizer.
+//
+//   b = post(branch) * post_weight + post_bias
+//   h = residual_scale * x + gate * b                       written in the rows' type
+//   z = (norm(h) * weight + bias) * (1 + scale) + shift     written in the rows' type, or as e4m3 codes and scales
+//
+// with post / norm the RMS or layer norm of a row, statistics and all arithmetic in fp32 from the unrounded h (one
+// rounding per output).  A row lives in registers between its loads and its stores, so each element is read once and
+// written once: the kernel is bound by HBM.  The layer norm takes its variance from the deviations (a second reduction
+// in registers), not from the difference of two sums.
+#include <type_traits>
+
+#include "sq_internal.h"
+#include "sq_rows.cuh"
+
+namespace sq {
+namespace {
+
+struct Param {      // rows of [width], `stride` elements apart, one for each `span` rows of x (span 0: one row for all)
+  const void* p;
+  int64_t stride;
+  uint32_t span;
+  int f32;
+};
+
+struct NormArgs {
+  const void* x;
+  const void* branch;
+  Param gate, post_weight, post_bias, weight, bias, mod_scale, mod_shift;
+  float residual_scale, eps;
+  int post_kind, norm_kind;
+  void* h_out;
+  void* z_out;
+  float* scales;
+  int64_t scales_row, scales_group;
+  int64_t rows;
+  int width;
+};
+
+// Sum over the TPR threads of a row, the same value in each of them and the same order in every run.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* partial) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  if (TPR > 32) {
+    const int warp = threadIdx.x >> 5;
+    __syncthreads();  // the last sum's readers are done with `partial`
+    if ((threadIdx.x & 31) == 0) partial[warp] = v;
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < TPR / 32; ++w) v += partial[w];
+  }
+  return v;
+}
+
+template <int VPT>
+__device__ __forceinline__ float local_squares(const float (&v)[VPT][8]) {
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf(v[i][e], v[i][e], s);
+  }
+  return s;
+}
+
+// v -> (v - mean) / sqrt(variance + eps) or v / sqrt(mean square + eps); slots without elements stay zero
+template <int TPR, int VPT>
+__device__ __forceinline__ void standardise(float (&v)[VPT][8], const bool (&on)[VPT], int kind, float eps, float inv_width,
+                                            float* partial) {
+  if (kind == SQ_NORM_LAYER) {
+    float share = 0.0f;  // of the mean: added up as v / width, which cannot overflow
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) share = fmaf(v[i][e], inv_width, share);
+    }
+    const float mean = row_sum<TPR>(share, partial);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = on[i] ? v[i][e] - mean : 0.0f;
+    }
+  }
+  float squares = row_sum<TPR>(local_squares(v), partial);
+  if (!(squares < __int_as_float(0x7F800000))) {
+    // the squares of bf16 values beyond 2^59 or so overflow: the row over again, 2^70 times smaller (eps is nothing next
+    // to such a row).  The sum is the same in every thread of the row, so all of them come here or none.
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] *= 8.470329472543003e-22f;
+    }
+    squares = row_sum<TPR>(local_squares(v), partial);
+    eps = 0.0f;
+  }
+  const float r = rsqrtf(fmaf(squares, inv_width, eps));
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[i][e] *= r;
+  }
+}
+
+// where a row's parameters start; computed once per row (a division)
+__device__ __forceinline__ int64_t param_base(const Param& q, int64_t row) {
+  return q.span > 0 ? static_cast<int64_t>(static_cast<uint32_t>(row) / q.span) * q.stride : 0;
+}
+template <typename T>
+__device__ __forceinline__ void params_at(const Param& q, int64_t base, int column, float (&v)[8]) {
+  load_params<T>(q.p, base + column, q.f32 != 0, v);
+}
+
+// TPR threads cover a row, thread t owning the vectors t, t + TPR, ... (VPT of them): a warp reads 512 contiguous
+// bytes, and the 16 vectors of a run of 128 sit in 16 neighbouring lanes.
+template <typename T, int TPR, int VPT, bool kBranch>
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) sq_block_norm_kernel(const NormArgs a) {
+  constexpr int kRowsPerBlock = TPR < 128 ? 128 / TPR : 1;
+  __shared__ float partial[TPR / 32];
+  const int t = threadIdx.x % TPR;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + threadIdx.x / TPR;
+  const bool row_on = row < a.rows;  // rows of a block past the last one: only where a warp is a row of its own
+  if (!row_on) return;
+  const T* tag = nullptr;
+  const int64_t base = row * a.width;
+  bool on[VPT];
+  uint4 raw_x[VPT], raw_b[kBranch ? VPT : 1];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int column = (t + i * TPR) * 8;
+    on[i] = column < a.width;
+    raw_x[i] = on[i] ? load_stream(static_cast<const T*>(a.x) + base + column) : make_uint4(0, 0, 0, 0);
+  }
+  if (kBranch) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      raw_b[i] = on[i] ? load_stream(static_cast<const T*>(a.branch) + base + (t + i * TPR) * 8) : make_uint4(0, 0, 0, 0);
+  }
+  const int64_t gate_base = kBranch ? param_base(a.gate, row) : 0;
+  const int64_t scale_base = param_base(a.mod_scale, row), shift_base = param_base(a.mod_shift, row);
+  const float inv_width = 1.0f / static_cast<float>(a.width);
+  float h[VPT][8];
+  float p[8];
+  if (kBranch) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) unpack8(raw_b[i], h[i], tag);
+    if (a.post_kind != SQ_NORM_NONE) {
+      standardise<TPR, VPT>(h, on, a.post_kind, a.eps, inv_width, partial);
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int column = (t + i * TPR) * 8;
+        if (!on[i]) continue;
+        if (a.post_weight.p != nullptr) {
+          params_at<T>(a.post_weight, 0, column, p);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) h[i][e] *= p[e];
+        }
+        if (a.post_bias.p != nullptr) {
+          params_at<T>(a.post_bias, 0, column, p);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) h[i][e] += p[e];
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int column = (t + i * TPR) * 8;
+      if (on[i] && a.gate.p != nullptr) {
+        params_at<T>(a.gate, gate_base, column, p);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[i][e] *= p[e];
+      }
+      float xv[8];
+      unpack8(raw_x[i], xv, tag);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[i][e] = fmaf(a.residual_scale, xv[e], h[i][e]);
+      if (on[i]) *reinterpret_cast<uint4*>(static_cast<T*>(a.h_out) + base + column) = pack8(h[i], tag);
+    }
+    if (a.norm_kind == SQ_NORM_NONE) return;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) unpack8(raw_x[i], h[i], tag);
+  }
+  standardise<TPR, VPT>(h, on, a.norm_kind, a.eps, inv_width, partial);
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int column = (t + i * TPR) * 8;
+    if (on[i]) {
+      if (a.weight.p != nullptr) {
+        params_at<T>(a.weight, 0, column, p);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[i][e] *= p[e];
+      }
+      if (a.bias.p != nullptr) {
+        params_at<T>(a.bias, 0, column, p);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[i][e] += p[e];
+      }
+      if (a.mod_scale.p != nullptr) {
+        params_at<T>(a.mod_scale, scale_base, column, p);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[i][e] = fmaf(h[i][e], p[e], h[i][e]);
+      }
+      if (a.mod_shift.p != nullptr) {
+        params_at<T>(a.mod_shift, shift_base, column, p);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[i][e] += p[e];
+      }
+      if (a.scales == nullptr) *reinterpret_cast<uint4*>(static_cast<T*>(a.z_out) + base + column) = pack8(h[i], tag);
+    }
+    if (a.scales != nullptr) {  // every lane of the warp is here: the run's maximum is a shuffle
+      const float s = e4m3_scale(run_max(on[i] ? magnitude8(h[i]) : 0u));
+      if (on[i]) {
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.z_out) + base + column) = quantize8(h[i], __fdiv_rn(1.0f, s));
+        if ((t & 15) == 0) a.scales[row * a.scales_row + (column >> 7) * a.scales_group] = s;
+      }
+    }
+  }
+}
+
+template <typename T, int TPR, int VPT>
+int launch_shape(const NormArgs& a, cudaStream_t stream) {
+  constexpr int kThreads = TPR < 128 ? 128 : TPR;
+  constexpr int kRowsPerBlock = kThreads / TPR;
+  const int64_t blocks = (a.rows + kRowsPerBlock - 1) / kRowsPerBlock;
+  if (a.branch != nullptr) sq_block_norm_kernel<T, TPR, VPT, true><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(a);
+  else sq_block_norm_kernel<T, TPR, VPT, false><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(a);
+  const cudaError_t err = cudaGetLastError();
+  return err == cudaSuccess ? SQ_OK : static_cast<int>(err);
+}
+
+// Threads per row and vectors per thread: a warp per row while a lane then holds at most four vectors, else the fewest
+// threads that hold the row in four vectors each.
+template <typename T>
+int launch_typed(const NormArgs& a, cudaStream_t stream) {
+  const int vectors = a.width / 8;
+  if (vectors <= 32) return launch_shape<T, 32, 1>(a, stream);
+  if (vectors <= 64) return launch_shape<T, 32, 2>(a, stream);
+  if (vectors <= 128) return launch_shape<T, 32, 4>(a, stream);
+  if (vectors <= 256) return launch_shape<T, 128, 2>(a, stream);
+  if (vectors <= 384) return launch_shape<T, 128, 3>(a, stream);
+  if (vectors <= 512) return launch_shape<T, 128, 4>(a, stream);
+  if (vectors <= 768) return launch_shape<T, 256, 3>(a, stream);
+  if (vectors <= 1024) return launch_shape<T, 256, 4>(a, stream);
+  if (vectors <= 1536) return launch_shape<T, 512, 3>(a, stream);
+  return launch_shape<T, 512, 4>(a, stream);
+}
+
+// ---------------------------------------------------------------------------------------------- e4m3 quantizer
+// 16 lanes per run of 128, kRuns runs per thread loaded before the first is used (64 bytes in flight per thread).  No row
+// statistics are needed, so runs are dealt out regardless of rows; the row of a run is a multiplication by the
+// reciprocal of the runs per row (exact for run numbers below 2^31).
+constexpr int kRuns = 4;
+constexpr int kQuantThreads = 256;
+
+template <typename T, bool kGelu>
+__global__ void __launch_bounds__(kQuantThreads) sq_fp8_quantize_kernel(
+    const T* __restrict__ x, uint8_t* __restrict__ codes, float* __restrict__ scales, int64_t scales_row,
+    int64_t scales_group, uint32_t runs, uint32_t runs_per_row, uint32_t magic, uint32_t shift, int width) {
+  // the product behind this kernel may set itself up meanwhile; it waits for this grid before it reads anything of it
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int lane16 = threadIdx.x & 15;
+  const uint32_t first = blockIdx.x * (kQuantThreads / 16 * kRuns) + (threadIdx.x >> 4);
+  uint4 raw[kRuns];
+  uint32_t row[kRuns], group[kRuns];
+  bool on[kRuns];
+#pragma unroll
+  for (int i = 0; i < kRuns; ++i) {
+    const uint32_t run = first + i * (kQuantThreads / 16);
+    row[i] = runs_per_row == 1 ? run : __umulhi(run, magic) >> shift;
+    group[i] = run - row[i] * runs_per_row;
+    const int column = static_cast<int>(group[i]) * 128 + lane16 * 8;
+    on[i] = run < runs && column < width;
+    raw[i] = on[i] ? load_stream(x + static_cast<int64_t>(row[i]) * width + column) : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < kRuns; ++i) {
+    float v[8];
+    unpack8(raw[i], v, static_cast<const T*>(nullptr));
+    if (kGelu) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = gelu_erf(v[e]);
+    }
+    const float s = e4m3_scale(run_max(magnitude8(v)));
+    if (on[i]) {
+      const int64_t at = static_cast<int64_t>(row[i]) * width + static_cast<int64_t>(group[i]) * 128 + lane16 * 8;
+      *reinterpret_cast<uint2*>(codes + at) = quantize8(v, __fdiv_rn(1.0f, s));
+      if (lane16 == 0) scales[static_cast<int64_t>(row[i]) * scales_row + static_cast<int64_t>(group[i]) * scales_group] = s;
+    }
+  }
+}
+
+}  // namespace
+
+int launch_fp8_quantize(const void* x, int x_dtype, int64_t rows, int64_t K, int input_activation, void* codes, float* scales,
+                        int64_t scales_row, int64_t scales_group, cudaStream_t stream) {
+  if (x == nullptr || codes == nullptr || scales == nullptr) return SQ_ERR_NULL;
+  if (x_dtype != SQ_BF16 && x_dtype != SQ_FP16) return SQ_ERR_ENUM;
+  if (input_activation != SQ_ACT_FN_NONE && input_activation != SQ_ACT_FN_GELU) return SQ_ERR_ENUM;
+  if (rows < 0 || K <= 0 || K % 16 != 0 || K > 131072) return SQ_ERR_SHAPE;
+  if (!aligned16_host(x) || !aligned16_host(codes) || (reinterpret_cast<uintptr_t>(scales) & 3u) != 0) return SQ_ERR_SHAPE;
+  if (rows == 0) return SQ_OK;
+  const int64_t per_row = (K + 127) / 128;
+  if (rows > (int64_t{1} << 30) / per_row) return SQ_ERR_SHAPE;
+  const uint32_t runs = static_cast<uint32_t>(rows * per_row);
+  // run / per_row = (run * magic) >> (32 + shift) with magic = ceil(2^(32 + shift) / per_row), 2^shift < per_row <=
+  // 2^(shift + 1): the error run * (magic * per_row - 2^(32 + shift)) stays below 2^(32 + shift) for run < 2^31
+  uint32_t shift = 0;
+  while ((int64_t{2} << shift) < per_row) ++shift;
+  const uint32_t magic = per_row == 1 ? 0 : static_cast<uint32_t>(((uint64_t{1} << (32 + shift)) + per_row - 1) / per_row);
+  const unsigned blocks = (runs + kQuantThreads / 16 * kRuns - 1) / (kQuantThreads / 16 * kRuns);
+  auto go = [&](auto tag, auto gelu) {
+    using T = decltype(tag);
+    sq_fp8_quantize_kernel<T, decltype(gelu)::value><<<blocks, kQuantThreads, 0, stream>>>(
+        static_cast<const T*>(x), static_cast<uint8_t*>(codes), scales, scales_row, scales_group, runs,
+        static_cast<uint32_t>(per_row), magic, shift, static_cast<int>(K));
+  };
+  const bool gelu = input_activation == SQ_ACT_FN_GELU;
+  if (x_dtype == SQ_BF16) gelu ? go(__nv_bfloat16{}, std::true_type{}) : go(__nv_bfloat16{}, std::false_type{});
+  else gelu ? go(__half{}, std::true_type{}) : go(__half{}, std::false_type{});
+  const cudaError_t err = cudaGetLastError();
+  return err == cudaSuccess ? SQ_OK : static_cast<int>(err);
+}
+
+int launch_block_norm(const SqBlockNorm& b, cudaStream_t stream) {
+  if (b.x == nullptr) return SQ_ERR_NULL;
+  if (b.dtype != SQ_BF16 && b.dtype != SQ_FP16) return SQ_ERR_ENUM;
+  for (const int kind : {b.post_kind, b.norm_kind})
+    if (kind != SQ_NORM_NONE && kind != SQ_NORM_LAYER && kind != SQ_NORM_RMS) return SQ_ERR_ENUM;
+  if (b.branch == nullptr && b.norm_kind == SQ_NORM_NONE) return SQ_ERR_NULL;
+  if ((b.branch != nullptr && b.h_out == nullptr) || (b.norm_kind != SQ_NORM_NONE && b.z_out == nullptr)) return SQ_ERR_NULL;
+  if (b.norm_kind == SQ_NORM_NONE && (b.scales != nullptr || b.mod_scale.data != nullptr || b.mod_shift.data != nullptr ||
+                                      b.weight.data != nullptr || b.bias.data != nullptr))
+    return SQ_ERR_ENUM;  // nothing would read them
+  if (b.branch == nullptr && (b.gate.data != nullptr || b.post_kind != SQ_NORM_NONE)) return SQ_ERR_ENUM;
+  if (b.post_kind == SQ_NORM_NONE && (b.post_weight.data != nullptr || b.post_bias.data != nullptr)) return SQ_ERR_ENUM;
+  if (b.rows < 0 || b.width <= 0 || b.width % (b.scales != nullptr ? 16 : 8) != 0 || b.width > 16384) return SQ_ERR_SHAPE;
+  if (b.rows > 0x7FFFFFFF) return SQ_ERR_SHAPE;
+  for (const void* p : {b.x, b.branch, static_cast<const void*>(b.h_out), static_cast<const void*>(b.z_out)})
+    if (!aligned16_host(p)) return SQ_ERR_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(b.scales) & 3u) != 0) return SQ_ERR_SHAPE;
+  NormArgs a = {};
+  // the per-channel vectors have one row; a span beyond the rows is one row too
+  auto row_of = [](const SqParam& q) { return Param{q.data, 0, 0u, q.is_fp32}; };
+  auto take = [&](const SqParam& q) {
+    return Param{q.data, q.row_stride, q.span >= b.rows ? 0u : static_cast<uint32_t>(q.span), q.is_fp32};
+  };
+  for (const SqParam* q : {&b.gate, &b.mod_scale, &b.mod_shift})
+    if (q->data != nullptr && (q->span <= 0 || q->row_stride < 0 || q->row_stride % 8 != 0)) return SQ_ERR_SHAPE;
+  a.gate = take(b.gate);
+  a.post_weight = row_of(b.post_weight);
+  a.post_bias = row_of(b.post_bias);
+  a.weight = row_of(b.weight);
+  a.bias = row_of(b.bias);
+  a.mod_scale = take(b.mod_scale);
+  a.mod_shift = take(b.mod_shift);
+  for (const Param& q : {a.gate, a.post_weight, a.post_bias, a.weight, a.bias, a.mod_scale, a.mod_shift})
+    if (!aligned16_host(q.p)) return SQ_ERR_SHAPE;  // vectors of 8 elements
+  if (b.rows == 0) return SQ_OK;
+  a.x = b.x;
+  a.branch = b.branch;
+  a.residual_scale = b.residual_scale;
+  a.eps = b.eps;
+  a.post_kind = b.post_kind;
+  a.norm_kind = b.norm_kind;
+  a.h_out = b.h_out;
+  a.z_out = b.z_out;
+  a.scales = b.scales;
+  a.scales_row = b.scales_row_stride;
+  a.scales_group = b.scales_group_stride;
+  a.rows = b.rows;
+  a.width = static_cast<int>(b.width);
+  return b.dtype == SQ_BF16 ? launch_typed<__nv_bfloat16>(a, stream) : launch_typed<__half>(a, stream);
+}
+
+}  // namespace sq

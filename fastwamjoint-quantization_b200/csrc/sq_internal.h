@@ -89,6 +89,28 @@ int launch_gemm_timeline(const GemmArgs& a, long long* timeline, cudaStream_t st
 // Tensor-pipe rate probe: n_cols in {64, 128, 256}; cycles is a device int64.
 int launch_mma_rate(int n_cols, int iters, long long* cycles, cudaStream_t stream);
 
+// 8-bit floating-point product with block scales (sq_fp8_gemm.cu).
+struct Fp8GemmArgs {
+  const void* codes;           // e4m3 [M, K]
+  const float* scales;         // [M, ceil(K / 128)], strides in elements
+  int64_t scales_row, scales_group;
+  const void* weight;          // e4m3 [N, K]
+  const float* weight_scales;  // [ceil(N / 128), ceil(K / 128)]
+  const void* bias;
+  void* out;
+  int out_dtype;
+  int64_t M, N, K;
+  bool after_quantize = false;  // launched right behind the quantizer that writes codes / scales: overlap the prologue
+};
+int validate_fp8_gemm(const Fp8GemmArgs& a);
+int launch_fp8_gemm(const Fp8GemmArgs& a, cudaStream_t stream);
+
+// Norms of a block, the e4m3 quantizer (sq_block_norm.cu) and rotary positions (sq_rotary.cu).
+int launch_fp8_quantize(const void* x, int x_dtype, int64_t rows, int64_t K, int input_activation, void* codes, float* scales,
+                        int64_t scales_row, int64_t scales_group, cudaStream_t stream);
+int launch_block_norm(const SqBlockNorm& b, cudaStream_t stream);
+int launch_rotary(const SqRotary& r, cudaStream_t stream);
+
 // One CTA waits `limit_us` for a barrier nobody arrives at, then reports status 9190 (see sq_wait_probe).
 int launch_wait_probe(int64_t limit_us, long long* waited_ns, cudaStream_t stream);
 

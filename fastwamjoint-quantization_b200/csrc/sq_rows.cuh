@@ -1,0 +1,113 @@
+// Row helpers shared by the block-norm, e4m3 quantizer and rotary kernels: 8-element vectors of bf16 / fp16 / fp32, e4m3
+// conversion with the scale of a run of 128, erf GELU.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace sq {
+
+constexpr float kE4M3Max = 448.0f;      // largest finite e4m3 value
+constexpr float kSmallestScale = 1e-8f; // floor of a scale: an all-zero run gets zero codes, not 0 / 0
+
+__device__ __forceinline__ void unpack8(const uint4& raw, float (&v)[8], const __nv_bfloat16*) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ void unpack8(const uint4& raw, float (&v)[8], const __half*) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ uint4 pack8(const float (&v)[8], const __nv_bfloat16*) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 pack8(const float (&v)[8], const __half*) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// data read once: past the L1, so that the parameter rows every token rereads stay there
+__device__ __forceinline__ uint4 load_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+
+// 8 parameters, in the rows' type or in fp32
+template <typename T>
+__device__ __forceinline__ void load_params(const void* base, int64_t index, bool f32, float (&v)[8]) {
+  if (f32) {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + index);
+    const float4 a = __ldg(p), b = __ldg(p + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+    unpack8(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(base) + index)), v, static_cast<const T*>(nullptr));
+  }
+}
+
+// Largest magnitude as an integer: magnitudes order like their bit patterns, and - unlike fmaxf - a NaN stays on top,
+// so a run that holds one gets a NaN scale and its row comes out NaN instead of silently finite.
+__device__ __forceinline__ uint32_t magnitude8(const float (&v)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  return m;
+}
+
+// Scale of a run of 128 from its largest magnitude: amax / 448, both divisions IEEE.  NaN stays NaN.
+__device__ __forceinline__ float e4m3_scale(uint32_t magnitude) {
+  const float s = __fdiv_rn(__uint_as_float(magnitude), kE4M3Max);
+  return s < kSmallestScale ? kSmallestScale : s;
+}
+
+// Four floats -> four e4m3 codes, round to nearest even, saturating (NaN gives the NaN code).
+__device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+  return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
+}
+
+// Codes of 8 elements given the run's scale: x * (1 / s), one reciprocal per run.
+__device__ __forceinline__ uint2 quantize8(const float (&v)[8], float inverse) {
+  return make_uint2(pack_e4m3x4(v[0] * inverse, v[1] * inverse, v[2] * inverse, v[3] * inverse),
+                    pack_e4m3x4(v[4] * inverse, v[5] * inverse, v[6] * inverse, v[7] * inverse));
+}
+
+// Largest magnitude over the 16 lanes (8 elements each) that hold a run of 128.
+__device__ __forceinline__ uint32_t run_max(uint32_t m) {
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+  return m;
+}
+
+__device__ __forceinline__ float gelu_erf(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f)); }
+
+inline bool aligned16_host(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+}  // namespace sq

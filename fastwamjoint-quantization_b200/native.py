@@ -250,6 +250,335 @@ def linear(x: torch.Tensor, packed: torch.Tensor, w_scales: torch.Tensor, bias, 
     return out
 
 
+# ---------------------------------------------------------------------------------------- operators of a block
+RUN = 128  # k that share a scale in the e4m3 product, and the rows of a weight block
+
+
+def _no_gradient(*tensors) -> None:
+    """The operators of this module are forward only.  An input that autograd tracks is refused: its gradient would
+    be lost without a word."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("the B200 operators have no backward pass: call them under torch.no_grad() or detach the inputs.")
+
+
+def _on_device(x: torch.Tensor, **others) -> None:
+    for name, t in others.items():
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name} must be on the input's device.")
+
+
+def _vectors(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous and 16-byte aligned (a copy where it is not): what the kernels read as vectors."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _require_rows(x: torch.Tensor, name: str = "x") -> None:
+    _require_cuda(x, name)
+    if x.dtype not in _DTYPES or x.ndim < 2:
+        raise ValueError(f"{name} must be a bf16 or fp16 tensor with token and channel axes.")
+
+
+def _input_activation(name: str | None) -> int:
+    if name not in (None, "gelu"):
+        raise ValueError("input_activation must be None or 'gelu'.")
+    return _lib.ACT_FN_GELU if name == "gelu" else _lib.ACT_FN_NONE
+
+
+def _scales_for(rows: int, width: int, device) -> torch.Tensor:
+    """fp32 [rows, runs] with the rows of a run next to each other, as the product reads them."""
+    return torch.empty((-(-width // RUN), rows), device=device, dtype=torch.float32).t()
+
+
+def fp8_quantize(x: torch.Tensor, *, input_activation: str | None = None):
+    """``x`` [..., tokens, K] bf16/fp16 -> ``(codes, scales)``: float8_e4m3fn of x's shape and fp32 [rows, ceil(K / 128)],
+    one scale per token and run of 128 channels (``max(amax / 448, 1e-8)``; codes are ``x * (1 / scale)`` rounded to
+    nearest even).  ``input_activation="gelu"`` applies the erf GELU first, in fp32.  K must be a multiple of 16."""
+    _require_rows(x)
+    _no_gradient(x)
+    activation = _input_activation(input_activation)
+    k = x.shape[-1]
+    if k == 0 or k % 16:
+        raise ValueError("the channel axis must be a positive multiple of 16.")
+    x = _vectors(x)
+    rows = x.numel() // k
+    codes = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
+    scales = _scales_for(rows, k, x.device)
+    with torch.cuda.device(x.device):
+        status = _lib.load_library().sq_fp8_quantize(x.data_ptr(), _DTYPES[x.dtype], rows, k, activation, codes.data_ptr(),
+                                                     scales.data_ptr(), scales.stride(0), scales.stride(1), _stream())
+    _lib.check(status, "sq_fp8_quantize")
+    return codes, scales
+
+
+def _check_fp8_weight(x: torch.Tensor, k: int, weight, weight_scales, bias, dtype) -> int:
+    _on_device(x, weight=weight, weight_scales=weight_scales, bias=bias)
+    if weight.dtype != torch.float8_e4m3fn or weight.ndim != 2 or not weight.is_contiguous() or weight.data_ptr() % 16:
+        raise ValueError("weight must be a contiguous, 16-byte aligned float8_e4m3fn [N, K] tensor.")
+    n = weight.shape[0]
+    if weight.shape[1] != k or k == 0 or k % 16 or n == 0 or n % 8:
+        raise ValueError(f"Unsupported e4m3 linear shape: K={k} (a multiple of 16), N={n} (a multiple of 8), weight {tuple(weight.shape)}.")
+    if weight_scales.dtype != torch.float32 or weight_scales.shape != (-(-n // RUN), -(-k // RUN)) or not weight_scales.is_contiguous():
+        raise ValueError("weight_scales must be contiguous float32 [ceil(N / 128), ceil(K / 128)].")
+    if bias is not None and (bias.dtype != dtype or bias.shape != (n,) or not bias.is_contiguous()):
+        raise ValueError("bias must be contiguous, [N], in the output's dtype.")
+    return n
+
+
+def _output(out, shape, dtype, device) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, device=device, dtype=dtype)
+    if out.shape != shape or out.dtype != dtype or out.device != device or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError(f"out must be a contiguous, 16-byte aligned {dtype} tensor of shape {tuple(shape)} on the input's device.")
+    return out
+
+
+def fp8_gemm(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor, bias=None, *,
+             out_dtype: torch.dtype, out: torch.Tensor | None = None) -> torch.Tensor:
+    """e4m3 codes [..., K] (with fp32 ``scales`` [rows, ceil(K / 128)], any strides) x e4m3 weight [N, K] (with fp32
+    ``weight_scales`` [ceil(N / 128), ceil(K / 128)], one per 128 x 128 block) + bias -> [..., N] in ``out_dtype``.  Sums in
+    fp32, one rounding.  ``quant.quantize_weight_block`` makes the weight's form, ``fp8_quantize`` the codes'."""
+    _require_cuda(codes, "codes")
+    _no_gradient(scales, weight_scales, bias, out)
+    if codes.dtype != torch.float8_e4m3fn or codes.ndim < 2:
+        raise ValueError("codes must be a float8_e4m3fn tensor with token and channel axes.")
+    if out_dtype not in _DTYPES:
+        raise ValueError("out_dtype must be torch.bfloat16 or torch.float16.")
+    _on_device(codes, scales=scales)
+    k = codes.shape[-1]
+    n = _check_fp8_weight(codes, k, weight, weight_scales, bias, out_dtype)
+    codes = _vectors(codes)
+    rows = codes.numel() // k
+    if scales.dtype != torch.float32 or scales.shape != (rows, -(-k // RUN)):
+        raise ValueError("scales must be float32 [rows, ceil(K / 128)].")
+    out = _output(out, (*codes.shape[:-1], n), out_dtype, codes.device)
+    if rows == 0:
+        return out
+    with torch.cuda.device(codes.device):
+        status = _lib.load_library().sq_fp8_gemm(codes.data_ptr(), scales.data_ptr(), scales.stride(0), scales.stride(1),
+                                                 weight.data_ptr(), weight_scales.data_ptr(), _ptr(bias), out.data_ptr(),
+                                                 _DTYPES[out_dtype], rows, n, k, _stream())
+    _lib.check(status, "sq_fp8_gemm")
+    return out
+
+
+def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor, bias=None, *,
+               input_activation: str | None = None, out: torch.Tensor | None = None,
+               workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """``linear([gelu](x))`` in e4m3: ``fp8_quantize`` and ``fp8_gemm`` as one call, the product's set-up and first weight
+    loads running under the quantizer.  ``workspace`` (uint8, at least ``sq_fp8_workspace_bytes(rows, K)``) may be passed
+    to reuse a buffer across calls that are ordered on the device; the weight must be ready before the call."""
+    _require_rows(x)
+    _no_gradient(x, weight_scales, bias, out)
+    activation = _input_activation(input_activation)
+    k = x.shape[-1]
+    n = _check_fp8_weight(x, k, weight, weight_scales, bias, x.dtype)
+    x = _vectors(x)
+    rows = x.numel() // k
+    lib = _lib.load_library()
+    nbytes = lib.sq_fp8_workspace_bytes(rows, k)
+    if workspace is None:
+        workspace = torch.empty((max(nbytes, 1),), device=x.device, dtype=torch.uint8)
+    elif (workspace.dtype != torch.uint8 or workspace.device != x.device or workspace.numel() < nbytes
+          or not workspace.is_contiguous() or workspace.data_ptr() % 16):
+        raise RuntimeError("workspace must be a contiguous, 16-byte aligned uint8 tensor on the input's device of at least "
+                           "sq_fp8_workspace_bytes(rows, K) bytes.")
+    out = _output(out, (*x.shape[:-1], n), x.dtype, x.device)
+    if rows == 0:
+        return out
+    with torch.cuda.device(x.device):
+        status = lib.sq_fp8_linear(x.data_ptr(), _DTYPES[x.dtype], rows, k, n, activation, weight.data_ptr(),
+                                   weight_scales.data_ptr(), _ptr(bias), out.data_ptr(), workspace.data_ptr(),
+                                   workspace.numel(), _stream())
+    _lib.check(status, "sq_fp8_linear")
+    return out
+
+
+def _param(t, x: torch.Tensor, rows: int, name: str, *, vector: bool = False):
+    """``(SqParam, tensor kept alive)`` of per-channel (``vector``) or per-group rows of parameters in x's dtype or fp32."""
+    if t is None:
+        return _lib.Param(), None
+    width = x.shape[-1]
+    if t.device != x.device or t.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"{name} must be on the input's device, in its dtype or float32.")
+    if vector:
+        if t.shape != (width,):
+            raise ValueError(f"{name} must be [{width}].")
+        t = _vectors(t)
+        return _lib.Param(t.data_ptr(), 0, 0, int(t.dtype == torch.float32), 0), t
+    if t.ndim < 1 or t.shape[-1] != width:
+        raise ValueError(f"{name} must have a last axis of {width} elements.")
+    t = t.reshape(-1, width)  # a view where the leading axes collapse to evenly spaced rows
+    groups = t.shape[0]
+    if rows and (groups == 0 or rows % groups):
+        raise ValueError(f"{name} rows must cover complete input rows: {groups} rows for {rows}.")
+    if t.stride(1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16:
+        t = _vectors(t)
+    return _lib.Param(t.data_ptr(), t.stride(0), max(rows // max(groups, 1), 1), int(t.dtype == torch.float32), 0), t
+
+
+_NORMS = {None: _lib.NORM_NONE, "layer": _lib.NORM_LAYER, "rms": _lib.NORM_RMS}
+
+
+def block_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *, gate=None, residual_scale: float = 1.0,
+               post_norm: str | None = None, post_weight=None, post_bias=None, norm: str | None = "rms", weight=None,
+               bias=None, mod_scale=None, mod_shift=None, eps: float = 1e-6, quantize: bool = False,
+               out: torch.Tensor | None = None):
+    """The norms around a block in one pass over its rows, returned as ``(h, z)``::
+
+        h = residual_scale * x + gate * (post_norm(branch) * post_weight + post_bias)
+        z = (norm(h) * weight + bias) * (1 + mod_scale) + mod_shift
+
+    ``x`` and ``branch`` are [..., width] bf16/fp16.  Without a ``branch`` h is x itself; with ``norm=None`` z is None.
+    Norms are "rms" or "layer", their statistics in fp32 from the unrounded h, both with ``eps``.  Weights and biases are
+    [width]; gate, mod_scale and mod_shift [..., width], each row for an equal share of x's rows (a strided slice of a
+    modulation table is read in place), all in x's dtype or fp32.  ``quantize`` gives z as ``(codes, scales)`` for
+    ``fp8_gemm`` (``fp8_quantize``'s rule, no rounding to x's dtype between).  ``out`` takes h; it may be x or branch."""
+    _require_rows(x)
+    _no_gradient(x, branch, gate, post_weight, post_bias, weight, bias, mod_scale, mod_shift, out)
+    if norm not in _NORMS or post_norm not in _NORMS:
+        raise ValueError("norm and post_norm must be None, 'rms' or 'layer'.")
+    if branch is None and (norm is None or gate is not None or post_norm is not None or residual_scale != 1.0 or out is not None):
+        raise ValueError("without a branch there is a norm alone: no gate, post_norm, residual_scale or out.")
+    if norm is None and (quantize or any(t is not None for t in (weight, bias, mod_scale, mod_shift))):
+        raise ValueError("without a norm there is nothing to weigh, modulate or quantize.")
+    if post_norm is None and (post_weight is not None or post_bias is not None):
+        raise ValueError("post_weight and post_bias belong to a post_norm.")
+    width = x.shape[-1]
+    if width == 0 or width % (16 if quantize else 8) or width > 16384:
+        raise ValueError("the channel axis must be a multiple of 8 (16 with quantize) up to 16384.")
+    if branch is not None and (branch.shape != x.shape or branch.dtype != x.dtype or branch.device != x.device):
+        raise ValueError("branch must match x's shape, dtype and device.")
+    x_rows = _vectors(x)
+    rows = x.numel() // width
+    args = _lib.BlockNorm(x=x_rows.data_ptr(), rows=rows, width=width, residual_scale=float(residual_scale), eps=float(eps),
+                          dtype=_DTYPES[x.dtype], post_kind=_NORMS[post_norm], norm_kind=_NORMS[norm])
+    kept = []
+    for name, t, vector in (("gate", gate, False), ("post_weight", post_weight, True), ("post_bias", post_bias, True),
+                            ("weight", weight, True), ("bias", bias, True), ("mod_scale", mod_scale, False),
+                            ("mod_shift", mod_shift, False)):
+        param, tensor = _param(t, x, rows, name, vector=vector)
+        setattr(args, name, param)
+        kept.append(tensor)
+    h, z = x, None
+    if branch is not None:
+        branch = _vectors(branch)
+        h = _output(out, x.shape, x.dtype, x.device)
+        args.branch, args.h_out = branch.data_ptr(), h.data_ptr()
+    if norm is not None:
+        z = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn if quantize else x.dtype)
+        args.z_out = z.data_ptr()
+        if quantize:
+            scales = _scales_for(rows, width, x.device)
+            args.scales, args.scales_row_stride, args.scales_group_stride = scales.data_ptr(), scales.stride(0), scales.stride(1)
+            z = (z, scales)
+    if rows == 0:
+        return h, z
+    with torch.cuda.device(x.device):
+        status = _lib.load_library().sq_block_norm(_lib.ctypes.byref(args), _stream())
+    _lib.check(status, "sq_block_norm")
+    return h, z
+
+
+_POSITIONS = {torch.int32: _lib.POS_INT32, torch.int64: _lib.POS_INT64, torch.float32: _lib.POS_FP32}
+_ROTARY_LAYOUTS = {"interleaved": _lib.ROTARY_INTERLEAVED, "half": _lib.ROTARY_HALF}
+_ROTARY_NORMS = {None: _lib.ROTARY_NORM_NONE, "head": _lib.ROTARY_NORM_HEAD, "token": _lib.ROTARY_NORM_TOKEN}
+
+
+def _heads_view(t: torch.Tensor, name: str) -> torch.Tensor:
+    """[batch, tokens, heads, dim] with vectors the kernel can read in place, or a copy that has them."""
+    if t.stride(3) == 1 and all(s % 8 == 0 for s in t.stride()[:3]) and t.data_ptr() % 16 == 0:
+        return t
+    return _vectors(t)
+
+
+def _heads_output(out, like: torch.Tensor, name: str) -> torch.Tensor:
+    if out is None:
+        return torch.empty(like.shape, device=like.device, dtype=like.dtype)
+    fits = (out.shape == like.shape and out.dtype == like.dtype and out.device == like.device and out.stride(3) == 1
+            and all(s % 8 == 0 and (s > 0 or n == 1) for s, n in zip(out.stride()[:3], out.shape)) and out.data_ptr() % 16 == 0)
+    if not fits:
+        raise ValueError(f"out for {name} must match it, with a contiguous last axis, strides that are multiples of 8 "
+                         "elements and 16-byte alignment.")
+    return out
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, *, sections,
+           layout: str = "interleaved", norm: str | None = None, q_weight=None, k_weight=None, eps: float = 1e-6, out=None):
+    """Rotary positions on several axes, with the q/k norm in front: returns ``(q, k)`` rotated.
+
+    ``q`` [batch, tokens, heads, dim] and ``k`` [batch, tokens, kv_heads, dim] (or None) bf16/fp16, strided views of a
+    packed projection read in place.  Pair j of every head turns by ``positions[..., axis] * inv_freq[j]`` radians;
+    ``sections`` are the pairs of each axis, in order (``rotary.rotary_frequencies`` makes inv_freq, float64 [pairs],
+    ``rotary.grid_positions`` the positions of a clip).  ``positions`` is [tokens, axes] or [batch, tokens, axes], int32,
+    int64 or float32, any value, however far or negative: angles are reduced in 64 bits (the rotation by
+    ``-positions`` undoes it).  ``layout``: pairs are neighbours ("interleaved") or half the rotated length apart
+    ("half"); elements past 2 * pairs pass through.  ``norm``: RMS of each head ("head", weights [dim]) or over all
+    heads of a token ("token", weights [heads * dim]).  ``out`` is a pair (q, k) of tensors to write, strided as a
+    cache or a transposed view may be; they may be the inputs themselves, but overlap nothing otherwise."""
+    for t, name in ((q, "q"), (k, "k")):
+        if t is None and name == "k":
+            continue
+        _require_cuda(t, name)
+        if t.ndim != 4 or t.dtype not in _DTYPES:
+            raise ValueError(f"{name} must be a bf16 or fp16 tensor [batch, tokens, heads, dim].")
+    out_q, out_k = out if out is not None else (None, None)
+    _no_gradient(q, k, q_weight, k_weight, inv_freq, positions, out_q, out_k)
+    batch, tokens, heads, dim = q.shape
+    if k is not None and (k.dtype != q.dtype or k.device != q.device or (k.shape[0], k.shape[1], k.shape[3]) != (batch, tokens, dim)):
+        raise ValueError("k must match q in dtype, device, batch, tokens and dim.")
+    if k is None and (k_weight is not None or out_k is not None):
+        raise ValueError("there is no k to weigh or to write.")
+    kv_heads = 0 if k is None else k.shape[2]
+    sections = tuple(int(s) for s in sections)
+    pairs = sum(sections)
+    if not 1 <= len(sections) <= _lib.ROTARY_AXES or min(sections) < 0 or pairs < 1 or 2 * pairs > dim:
+        raise ValueError(f"sections must be the pairs of 1 to {_lib.ROTARY_AXES} axes, at most dim / 2 together.")
+    lanes = 1 << max(dim // 8 - 1, 0).bit_length()
+    if dim % 8 or not 8 <= dim <= 256 or heads == 0 or (k is not None and kv_heads == 0) or (heads + kv_heads) * lanes > 4096:
+        raise ValueError(f"Unsupported head shape: {heads} + {kv_heads} heads of {dim}.")
+    if layout not in _ROTARY_LAYOUTS or norm not in _ROTARY_NORMS:
+        raise ValueError("layout must be 'interleaved' or 'half', norm None, 'head' or 'token'.")
+    if norm is None and (q_weight is not None or k_weight is not None):
+        raise ValueError("q_weight and k_weight belong to a norm.")
+    _on_device(q, positions=positions, inv_freq=inv_freq, q_weight=q_weight, k_weight=k_weight)
+    if inv_freq.dtype != torch.float64 or inv_freq.shape != (pairs,) or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq must be contiguous float64 [pairs].")
+    if (positions.dtype not in _POSITIONS or positions.ndim not in (2, 3) or positions.shape[-2:] != (tokens, len(sections))
+            or (positions.ndim == 3 and positions.shape[0] not in (1, batch))):
+        raise ValueError("positions must be int32, int64 or float32 [tokens, axes] or [batch, tokens, axes].")
+    if positions.stride(-1) != 1:
+        positions = positions.contiguous()
+    weights = []
+    for t, name, count in ((q_weight, "q_weight", heads), (k_weight, "k_weight", kv_heads)):
+        if t is not None:
+            if t.dtype not in (q.dtype, torch.float32) or t.shape != ((count * dim,) if norm == "token" else (dim,)):
+                raise ValueError(f"{name} must be [dim] (head norm) or [heads * dim] (token norm), in q's dtype or float32.")
+            t = _vectors(t)
+        weights.append(t)
+    q_in, k_in = _heads_view(q, "q"), None if k is None else _heads_view(k, "k")
+    q_out = _heads_output(out_q, q, "q")
+    k_out = None if k is None else _heads_output(out_k, k, "k")
+    if batch * tokens == 0:
+        return q_out, k_out
+    three = lambda t: (0, 0, 0) if t is None else t.stride()[:3]
+    args = _lib.Rotary(q=q_in.data_ptr(), k=_ptr(k_in), q_out=q_out.data_ptr(), k_out=_ptr(k_out),
+                       q_weight=_ptr(weights[0]), k_weight=_ptr(weights[1]), positions=positions.data_ptr(),
+                       position_batch_stride=positions.stride(0) if positions.ndim == 3 and positions.shape[0] > 1 else 0,
+                       position_token_stride=positions.stride(-2), inv_freq=inv_freq.data_ptr(), batch=batch, length=tokens,
+                       heads=heads, kv_heads=kv_heads, dim=dim, axes=len(sections), dtype=_DTYPES[q.dtype],
+                       layout=_ROTARY_LAYOUTS[layout], norm=_ROTARY_NORMS[norm], position_type=_POSITIONS[positions.dtype],
+                       q_weight_fp32=int(weights[0] is not None and weights[0].dtype == torch.float32),
+                       k_weight_fp32=int(weights[1] is not None and weights[1].dtype == torch.float32), eps=float(eps))
+    args.q_strides[:], args.k_strides[:] = three(q_in), three(k_in)
+    args.q_out_strides[:], args.k_out_strides[:] = three(q_out), three(k_out)
+    args.sections[:len(sections)] = sections
+    with torch.cuda.device(q.device):
+        status = _lib.load_library().sq_rotary(_lib.ctypes.byref(args), _stream())
+    _lib.check(status, "sq_rotary")
+    return q_out, k_out
+
+
 TIMELINE_ROLES = ("tma_issue", "unpack_start", "unpack_done", "acc_free", "mma_issue", "drain_start",
                   "acc_released", "drain_done", "mma_committed", "drain_top", "acc_loaded", "item_end")
 

@@ -4,8 +4,11 @@ benchmark configurations use.  These run once at load time, not on the hot path.
 from __future__ import annotations
 
 import torch
+import torch.nn.functional as F
 
 GROUP = 128
+E4M3_MAX = 448.0  # largest finite float8_e4m3fn value
+SMALLEST_SCALE = 1e-8
 
 
 def _qmax(bits: int) -> int:
@@ -66,3 +69,45 @@ def quantize_weight_group(weight: torch.Tensor, *, bits: int = 4, group: int = G
     scales = scales.clamp_min(torch.finfo(torch.float16).tiny)
     codes = (rows / scales.float()).round().clamp(-limit, limit).to(torch.int8)
     return codes.reshape(n, k), scales.reshape(n, k // group)
+
+
+def _blocks(n: int) -> int:
+    return -(-n // GROUP)
+
+
+def quantize_weight_block(weight: torch.Tensor):
+    """float8_e4m3fn codes ``[N, K]`` and fp32 scales ``[ceil(N / 128), ceil(K / 128)]``, one for each 128 x 128 block of
+    the weight: ``max(amax / 448, 1e-8)``, the form ``native.fp8_gemm`` takes."""
+    if weight.ndim != 2:
+        raise ValueError("weight must be [N, K].")
+    n, k = weight.shape
+    padded = torch.zeros(_blocks(n) * GROUP, _blocks(k) * GROUP, device=weight.device)
+    padded[:n, :k] = weight.detach().float()
+    blocks = padded.view(_blocks(n), GROUP, _blocks(k), GROUP)
+    amax = blocks.abs().amax(dim=(1, 3))
+    scales = (amax / torch.full_like(amax, E4M3_MAX)).clamp_min(SMALLEST_SCALE)
+    codes = (blocks / scales[:, None, :, None]).clamp(-E4M3_MAX, E4M3_MAX).view(padded.shape)[:n, :k]
+    return codes.to(torch.float8_e4m3fn).contiguous(), scales.contiguous()
+
+
+def dequantize_weight_block(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """fp32 ``[N, K]`` values of ``quantize_weight_block``'s form."""
+    n, k = codes.shape
+    return codes.float() * scales.repeat_interleave(GROUP, dim=0)[:n].repeat_interleave(GROUP, dim=1)[:, :k]
+
+
+def quantize_token_runs(values: torch.Tensor):
+    """float8_e4m3fn codes of ``values`` [rows, K] and fp32 scales [rows, ceil(K / 128)]: ``native.fp8_quantize``'s rule
+    (``max(amax / 448, 1e-8)`` per run of 128, codes from one reciprocal per run) in plain torch."""
+    rows, k = values.shape
+    runs = F.pad(values.float(), (0, _blocks(k) * GROUP - k)).view(rows, _blocks(k), GROUP)
+    amax = runs.abs().amax(dim=2)
+    scales = (amax / torch.full_like(amax, E4M3_MAX)).clamp_min(SMALLEST_SCALE)
+    codes = (runs * scales.reciprocal()[:, :, None]).clamp(-E4M3_MAX, E4M3_MAX)
+    return codes.to(torch.float8_e4m3fn).view(rows, -1)[:, :k], scales
+
+
+def fake_quant_token_runs(values: torch.Tensor) -> torch.Tensor:
+    """Quantize-dequantize of ``quantize_token_runs``: fp32 [rows, K]."""
+    codes, scales = quantize_token_runs(values)
+    return codes.float() * scales.repeat_interleave(GROUP, dim=1)[:, :values.shape[1]]

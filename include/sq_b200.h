@@ -286,6 +286,101 @@ int sq_linear_noalloc(const void* x, int x_dtype, int64_t rows, int64_t K, int64
                       const void* w_packed, const void* w_scales, int wscale_mode, const void* bias,
                       void* out, void* stream);
 
+/* ---- Operators of a transformer block beside the int4 linears (no counterpart in the reference) ---- */
+
+/* Activations to e4m3: x [rows, K] bf16 / fp16 (x_dtype) -> codes [rows, K] and one fp32 scale per row and run of 128 k
+ * (the last run may be shorter): scale = max(amax / 448, 1e-8), code = e4m3(x * (1 / scale)), round to nearest even,
+ * saturating.  A run with a NaN or an infinity gets a scale of that kind and its row of a product comes out NaN.
+ * scales[row, run] lies at row * scales_row_stride + run * scales_group_stride.  input_activation: SQ_ACT_FN_GELU applies
+ * the erf GELU in fp32 first.  K % 16 == 0, K <= 131072; x and codes 16-byte aligned. */
+int sq_fp8_quantize(const void* x, int x_dtype, int64_t rows, int64_t K, int input_activation, void* codes, float* scales,
+                    int64_t scales_row_stride, int64_t scales_group_stride, void* stream);
+
+/* out[m, n] = sum over runs g of 128 k of scales[m, g] * weight_scales[n / 128, g] * (codes[m, :] . weight[n, :] in g)
+ * + bias[n], all of it in fp32 and rounded once to out_dtype.  codes e4m3 [M, K], weight e4m3 [N, K], weight_scales fp32
+ * [ceil(N / 128), ceil(K / 128)], bias [N] in out's type or null, out [M, N].
+ * N % 8 == 0, K % 16 == 0, K <= 131072; codes, weight and out 16-byte aligned.  The result does not depend on
+ * anything but the inputs (no atomics). */
+int sq_fp8_gemm(const void* codes, const float* scales, int64_t scales_row_stride, int64_t scales_group_stride,
+                const void* weight, const float* weight_scales, const void* bias, void* out, int out_dtype, int64_t M,
+                int64_t N, int64_t K, void* stream);
+
+/* sq_fp8_quantize into `workspace` (at least sq_fp8_workspace_bytes(rows, K), 16-byte aligned), then sq_fp8_gemm, whose
+ * set-up and first weight loads overlap the quantizer: the weight must not be written by it. */
+int sq_fp8_linear(const void* x, int x_dtype, int64_t rows, int64_t K, int64_t N, int input_activation, const void* weight,
+                  const float* weight_scales, const void* bias, void* out, void* workspace, size_t workspace_bytes,
+                  void* stream);
+size_t sq_fp8_workspace_bytes(int64_t rows, int64_t K);
+
+/* Rows of parameters: [width] elements in the rows' type (is_fp32 = 0) or fp32, 16-byte aligned; data null: absent. */
+typedef struct SqParam {
+  const void* data;
+  int64_t row_stride; /* elements between rows (a multiple of 8); ignored for per-channel vectors */
+  int64_t span;       /* rows of x per row of parameters (>= 1); ignored for per-channel vectors */
+  int32_t is_fp32;
+  int32_t reserved;
+} SqParam;
+
+/* The norms before and after a block with its gate and residual scale:
+ *   b = post(branch) * post_weight + post_bias
+ *   h = residual_scale * x + gate * b                      -> h_out, in x's type (may be x or branch itself)
+ *   z = (norm(h) * weight + bias) * (1 + mod_scale) + mod_shift  -> z_out
+ * post_kind / norm_kind: SQ_NORM_NONE, SQ_NORM_LAYER or SQ_NORM_RMS over the row, fp32 statistics of the unrounded h.
+ * branch null: h is x, nothing is written to h_out.  norm_kind none: only h.  scales null: z in x's type; else z_out takes
+ * e4m3 codes and scales one fp32 per row and run of 128 (sq_fp8_quantize's rule).  width % 8 == 0 (16 with scales),
+ * width <= 16384; x, branch, h_out, z_out [rows, width], 16-byte aligned. */
+typedef struct SqBlockNorm {
+  const void* x;
+  const void* branch;
+  SqParam gate, post_weight, post_bias, weight, bias, mod_scale, mod_shift;
+  void* h_out;
+  void* z_out;
+  float* scales;
+  int64_t scales_row_stride, scales_group_stride;
+  int64_t rows, width;
+  float residual_scale, eps;
+  int32_t dtype, post_kind, norm_kind;
+  int32_t reserved;
+} SqBlockNorm;
+int sq_block_norm(const SqBlockNorm* args_host, void* stream);
+
+/* Rotary positions on up to SQ_ROTARY_AXES axes.  q [batch, length, heads, dim], k [batch, length, kv_heads, dim] with
+ * any strides that are multiples of 8 elements (innermost contiguous); the outputs may be the inputs.  Pair j of a head
+ * turns by positions[b, t, axis(j)] * inv_freq[j] radians (reduced in 64 bits); the pairs are dealt to the axes in
+ * order, sections[x] of them to axis x.  layout: pairs (2j, 2j + 1) or (j, j + pairs); elements past 2 * pairs stay.
+ * norm: RMS over each head, or over all heads of a token, in front; weights [dim], or [heads * dim] for the token norm,
+ * null for none.  dim % 8 == 0, dim <= 256; (heads + kv_heads) * (dim / 8 up to a power of two) <= 4096.
+ * k null with kv_heads = 0: q alone.  The axes of a token's positions are neighbours. */
+#define SQ_ROTARY_AXES 4
+#define SQ_ROTARY_INTERLEAVED 0
+#define SQ_ROTARY_HALF 1
+#define SQ_ROTARY_NORM_NONE 0
+#define SQ_ROTARY_NORM_HEAD 1
+#define SQ_ROTARY_NORM_TOKEN 2
+#define SQ_POS_INT32 0
+#define SQ_POS_INT64 1
+#define SQ_POS_FP32 2
+typedef struct SqRotary {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  int64_t q_strides[3], k_strides[3], q_out_strides[3], k_out_strides[3]; /* batch, token, head; elements */
+  const void* q_weight;
+  const void* k_weight;
+  const void* positions;
+  int64_t position_batch_stride, position_token_stride; /* elements */
+  const double* inv_freq;                                /* [pairs] */
+  int64_t batch, length;
+  int32_t heads, kv_heads, dim, axes;
+  int32_t sections[SQ_ROTARY_AXES];
+  int32_t dtype, layout, norm, position_type;
+  int32_t q_weight_fp32, k_weight_fp32;
+  float eps;
+  int32_t reserved;
+} SqRotary;
+int sq_rotary(const SqRotary* args_host, void* stream);
+
 /* Test aid with no counterpart in the reference: proves that a wait which runs out ends as a status, not as a hung
  * GPU.  One thread block allocates tensor memory, waits at most `limit_us` microseconds (1 ... 100000) on a barrier
  * nobody ever arrives at - through the same bounded wait every pipeline role of sq_gemm uses, whose own limit is
