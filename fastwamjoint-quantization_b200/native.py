@@ -251,20 +251,32 @@ def linear(x: torch.Tensor, packed: torch.Tensor, w_scales: torch.Tensor, bias, 
 
 
 # ---------------------------------------------------------------------------------------- operators of a block
+# The smallest calls of these operators take 3 us on the device, so what the host does per call is their cost: properties
+# are read once, arguments go to C as one structure filled by position, the stream is asked for by device index.
 RUN = 128  # k that share a scale in the e4m3 product, and the rows of a weight block
+_E4M3 = torch.float8_e4m3fn
 
 
 def _no_gradient(*tensors) -> None:
-    """The operators of this module are forward only.  An input that autograd tracks is refused: its gradient would
-    be lost without a word."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("the B200 operators have no backward pass: call them under torch.no_grad() or detach the inputs.")
+    """The operators below are forward only.  An input that autograd tracks is refused: its gradient would be lost
+    without a word."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("the B200 operators have no backward pass: call them under torch.no_grad() or detach the inputs.")
 
 
-def _on_device(x: torch.Tensor, **others) -> None:
-    for name, t in others.items():
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{name} must be on the input's device.")
+def _call(name: str, device: torch.device, *args) -> None:
+    """One C entry point on ``device`` and its current stream."""
+    fn = getattr(_lib.load_library(), name)
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status, name)
 
 
 def _vectors(t: torch.Tensor) -> torch.Tensor:
@@ -274,20 +286,24 @@ def _vectors(t: torch.Tensor) -> torch.Tensor:
 
 
 def _require_rows(x: torch.Tensor, name: str = "x") -> None:
-    _require_cuda(x, name)
+    if not x.is_cuda:
+        _require_cuda(x, name)
     if x.dtype not in _DTYPES or x.ndim < 2:
         raise ValueError(f"{name} must be a bf16 or fp16 tensor with token and channel axes.")
 
 
+_ACTIVATIONS = {None: _lib.ACT_FN_NONE, "gelu": _lib.ACT_FN_GELU}
+
+
 def _input_activation(name: str | None) -> int:
-    if name not in (None, "gelu"):
+    if name not in _ACTIVATIONS:
         raise ValueError("input_activation must be None or 'gelu'.")
-    return _lib.ACT_FN_GELU if name == "gelu" else _lib.ACT_FN_NONE
+    return _ACTIVATIONS[name]
 
 
 def _scales_for(rows: int, width: int, device) -> torch.Tensor:
     """fp32 [rows, runs] with the rows of a run next to each other, as the product reads them."""
-    return torch.empty((-(-width // RUN), rows), device=device, dtype=torch.float32).t()
+    return torch.empty_strided((rows, -(-width // RUN)), (1, max(rows, 1)), dtype=torch.float32, device=device)
 
 
 def fp8_quantize(x: torch.Tensor, *, input_activation: str | None = None):
@@ -301,33 +317,31 @@ def fp8_quantize(x: torch.Tensor, *, input_activation: str | None = None):
     if k == 0 or k % 16:
         raise ValueError("the channel axis must be a positive multiple of 16.")
     x = _vectors(x)
+    device = x.device
     rows = x.numel() // k
-    codes = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
-    scales = _scales_for(rows, k, x.device)
-    with torch.cuda.device(x.device):
-        status = _lib.load_library().sq_fp8_quantize(x.data_ptr(), _DTYPES[x.dtype], rows, k, activation, codes.data_ptr(),
-                                                     scales.data_ptr(), scales.stride(0), scales.stride(1), _stream())
-    _lib.check(status, "sq_fp8_quantize")
+    codes = torch.empty_like(x, dtype=_E4M3)
+    scales = _scales_for(rows, k, device)
+    _call("sq_fp8_quantize", device, x.data_ptr(), _DTYPES[x.dtype], rows, k, activation, codes.data_ptr(),
+          scales.data_ptr(), 1, max(rows, 1))
     return codes, scales
 
 
-def _check_fp8_weight(x: torch.Tensor, k: int, weight, weight_scales, bias, dtype) -> int:
-    _on_device(x, weight=weight, weight_scales=weight_scales, bias=bias)
-    if weight.dtype != torch.float8_e4m3fn or weight.ndim != 2 or not weight.is_contiguous() or weight.data_ptr() % 16:
+def _check_fp8_weight(device, k: int, weight, weight_scales, bias, dtype) -> int:
+    if weight.device != device or weight_scales.device != device or (bias is not None and bias.device != device):
+        raise ValueError("weight, weight_scales and bias must be on the input's device.")
+    if weight.dtype is not _E4M3 or weight.ndim != 2 or not weight.is_contiguous() or weight.data_ptr() % 16:
         raise ValueError("weight must be a contiguous, 16-byte aligned float8_e4m3fn [N, K] tensor.")
-    n = weight.shape[0]
-    if weight.shape[1] != k or k == 0 or k % 16 or n == 0 or n % 8:
-        raise ValueError(f"Unsupported e4m3 linear shape: K={k} (a multiple of 16), N={n} (a multiple of 8), weight {tuple(weight.shape)}.")
-    if weight_scales.dtype != torch.float32 or weight_scales.shape != (-(-n // RUN), -(-k // RUN)) or not weight_scales.is_contiguous():
+    n, width = weight.shape
+    if width != k or k == 0 or k % 16 or n == 0 or n % 8:
+        raise ValueError(f"Unsupported e4m3 linear shape: K={k} (a multiple of 16), N={n} (a multiple of 8), weight {(n, width)}.")
+    if weight_scales.dtype is not torch.float32 or weight_scales.shape != (-(-n // RUN), -(-k // RUN)) or not weight_scales.is_contiguous():
         raise ValueError("weight_scales must be contiguous float32 [ceil(N / 128), ceil(K / 128)].")
-    if bias is not None and (bias.dtype != dtype or bias.shape != (n,) or not bias.is_contiguous()):
+    if bias is not None and (bias.dtype is not dtype or bias.shape != (n,) or not bias.is_contiguous()):
         raise ValueError("bias must be contiguous, [N], in the output's dtype.")
     return n
 
 
-def _output(out, shape, dtype, device) -> torch.Tensor:
-    if out is None:
-        return torch.empty(shape, device=device, dtype=dtype)
+def _checked_output(out, shape, dtype, device) -> torch.Tensor:
     if out.shape != shape or out.dtype != dtype or out.device != device or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError(f"out must be a contiguous, 16-byte aligned {dtype} tensor of shape {tuple(shape)} on the input's device.")
     return out
@@ -338,27 +352,27 @@ def fp8_gemm(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, we
     """e4m3 codes [..., K] (with fp32 ``scales`` [rows, ceil(K / 128)], any strides) x e4m3 weight [N, K] (with fp32
     ``weight_scales`` [ceil(N / 128), ceil(K / 128)], one per 128 x 128 block) + bias -> [..., N] in ``out_dtype``.  Sums in
     fp32, one rounding.  ``quant.quantize_weight_block`` makes the weight's form, ``fp8_quantize`` the codes'."""
-    _require_cuda(codes, "codes")
+    if not codes.is_cuda:
+        _require_cuda(codes, "codes")
     _no_gradient(scales, weight_scales, bias, out)
-    if codes.dtype != torch.float8_e4m3fn or codes.ndim < 2:
+    if codes.dtype is not _E4M3 or codes.ndim < 2:
         raise ValueError("codes must be a float8_e4m3fn tensor with token and channel axes.")
     if out_dtype not in _DTYPES:
         raise ValueError("out_dtype must be torch.bfloat16 or torch.float16.")
-    _on_device(codes, scales=scales)
-    k = codes.shape[-1]
-    n = _check_fp8_weight(codes, k, weight, weight_scales, bias, out_dtype)
+    device = codes.device
+    shape = codes.shape
+    k = shape[-1]
+    n = _check_fp8_weight(device, k, weight, weight_scales, bias, out_dtype)
     codes = _vectors(codes)
     rows = codes.numel() // k
-    if scales.dtype != torch.float32 or scales.shape != (rows, -(-k // RUN)):
-        raise ValueError("scales must be float32 [rows, ceil(K / 128)].")
-    out = _output(out, (*codes.shape[:-1], n), out_dtype, codes.device)
-    if rows == 0:
-        return out
-    with torch.cuda.device(codes.device):
-        status = _lib.load_library().sq_fp8_gemm(codes.data_ptr(), scales.data_ptr(), scales.stride(0), scales.stride(1),
-                                                 weight.data_ptr(), weight_scales.data_ptr(), _ptr(bias), out.data_ptr(),
-                                                 _DTYPES[out_dtype], rows, n, k, _stream())
-    _lib.check(status, "sq_fp8_gemm")
+    if scales.dtype is not torch.float32 or scales.device != device or scales.shape != (rows, -(-k // RUN)):
+        raise ValueError("scales must be float32 [rows, ceil(K / 128)] on the codes' device.")
+    out_shape = (*shape[:-1], n)
+    out = codes.new_empty(out_shape, dtype=out_dtype) if out is None else _checked_output(out, out_shape, out_dtype, device)
+    if rows:
+        row_stride, run_stride = scales.stride()
+        _call("sq_fp8_gemm", device, codes.data_ptr(), scales.data_ptr(), row_stride, run_stride, weight.data_ptr(),
+              weight_scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), _DTYPES[out_dtype], rows, n, k)
     return out
 
 
@@ -371,50 +385,68 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tenso
     _require_rows(x)
     _no_gradient(x, weight_scales, bias, out)
     activation = _input_activation(input_activation)
-    k = x.shape[-1]
-    n = _check_fp8_weight(x, k, weight, weight_scales, bias, x.dtype)
+    device, shape, dtype = x.device, x.shape, x.dtype
+    k = shape[-1]
+    n = _check_fp8_weight(device, k, weight, weight_scales, bias, dtype)
     x = _vectors(x)
     rows = x.numel() // k
-    lib = _lib.load_library()
-    nbytes = lib.sq_fp8_workspace_bytes(rows, k)
+    nbytes = _lib.load_library().sq_fp8_workspace_bytes(rows, k)
     if workspace is None:
-        workspace = torch.empty((max(nbytes, 1),), device=x.device, dtype=torch.uint8)
-    elif (workspace.dtype != torch.uint8 or workspace.device != x.device or workspace.numel() < nbytes
+        workspace = x.new_empty((nbytes,), dtype=torch.uint8)
+    elif (workspace.dtype != torch.uint8 or workspace.device != device or workspace.numel() < nbytes
           or not workspace.is_contiguous() or workspace.data_ptr() % 16):
         raise RuntimeError("workspace must be a contiguous, 16-byte aligned uint8 tensor on the input's device of at least "
                            "sq_fp8_workspace_bytes(rows, K) bytes.")
-    out = _output(out, (*x.shape[:-1], n), x.dtype, x.device)
-    if rows == 0:
-        return out
-    with torch.cuda.device(x.device):
-        status = lib.sq_fp8_linear(x.data_ptr(), _DTYPES[x.dtype], rows, k, n, activation, weight.data_ptr(),
-                                   weight_scales.data_ptr(), _ptr(bias), out.data_ptr(), workspace.data_ptr(),
-                                   workspace.numel(), _stream())
-    _lib.check(status, "sq_fp8_linear")
+    out_shape = (*shape[:-1], n)
+    out = x.new_empty(out_shape) if out is None else _checked_output(out, out_shape, dtype, device)
+    if rows:
+        _call("sq_fp8_linear", device, x.data_ptr(), _DTYPES[dtype], rows, k, n, activation, weight.data_ptr(),
+              weight_scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), workspace.data_ptr(), nbytes)
     return out
 
 
-def _param(t, x: torch.Tensor, rows: int, name: str, *, vector: bool = False):
-    """``(SqParam, tensor kept alive)`` of per-channel (``vector``) or per-group rows of parameters in x's dtype or fp32."""
+_ABSENT = (0, 0, 0, 0, 0)
+
+
+def _channel_param(t, kept: list, width: int, dtype, device, name: str):
+    """Fields of an ``SqParam`` for a [width] vector in the rows' dtype or fp32."""
     if t is None:
-        return _lib.Param(), None
-    width = x.shape[-1]
-    if t.device != x.device or t.dtype not in (x.dtype, torch.float32):
+        return _ABSENT
+    f32 = t.dtype is torch.float32
+    if t.device != device or not (f32 or t.dtype is dtype):
         raise ValueError(f"{name} must be on the input's device, in its dtype or float32.")
-    if vector:
-        if t.shape != (width,):
-            raise ValueError(f"{name} must be [{width}].")
+    if t.shape != (width,):
+        raise ValueError(f"{name} must be [{width}].")
+    pointer = t.data_ptr()
+    if pointer % 16 or not t.is_contiguous():
         t = _vectors(t)
-        return _lib.Param(t.data_ptr(), 0, 0, int(t.dtype == torch.float32), 0), t
+        kept.append(t)
+        pointer = t.data_ptr()
+    return (pointer, 0, 0, f32, 0)
+
+
+def _row_param(t, kept: list, rows: int, width: int, dtype, device, name: str):
+    """The same for rows of parameters, each for an equal share of the input rows."""
+    if t is None:
+        return _ABSENT
+    f32 = t.dtype is torch.float32
+    if t.device != device or not (f32 or t.dtype is dtype):
+        raise ValueError(f"{name} must be on the input's device, in its dtype or float32.")
     if t.ndim < 1 or t.shape[-1] != width:
         raise ValueError(f"{name} must have a last axis of {width} elements.")
-    t = t.reshape(-1, width)  # a view where the leading axes collapse to evenly spaced rows
+    if t.ndim != 2:
+        t = t.reshape(-1, width)  # a view where the leading axes collapse to evenly spaced rows
+        kept.append(t)
     groups = t.shape[0]
     if rows and (groups == 0 or rows % groups):
         raise ValueError(f"{name} rows must cover complete input rows: {groups} rows for {rows}.")
-    if t.stride(1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16:
+    stride, step = t.stride()
+    pointer = t.data_ptr()
+    if step != 1 or stride % 8 or pointer % 16:
         t = _vectors(t)
-    return _lib.Param(t.data_ptr(), t.stride(0), max(rows // max(groups, 1), 1), int(t.dtype == torch.float32), 0), t
+        kept.append(t)
+        pointer, stride = t.data_ptr(), width
+    return (pointer, stride, rows // groups if rows else 1, f32, 0)
 
 
 _NORMS = {None: _lib.NORM_NONE, "layer": _lib.NORM_LAYER, "rms": _lib.NORM_RMS}
@@ -444,63 +476,84 @@ def block_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *, gate=None
         raise ValueError("without a norm there is nothing to weigh, modulate or quantize.")
     if post_norm is None and (post_weight is not None or post_bias is not None):
         raise ValueError("post_weight and post_bias belong to a post_norm.")
-    width = x.shape[-1]
+    device, shape, dtype = x.device, x.shape, x.dtype
+    width = shape[-1]
     if width == 0 or width % (16 if quantize else 8) or width > 16384:
         raise ValueError("the channel axis must be a multiple of 8 (16 with quantize) up to 16384.")
-    if branch is not None and (branch.shape != x.shape or branch.dtype != x.dtype or branch.device != x.device):
-        raise ValueError("branch must match x's shape, dtype and device.")
     x_rows = _vectors(x)
     rows = x.numel() // width
-    args = _lib.BlockNorm(x=x_rows.data_ptr(), rows=rows, width=width, residual_scale=float(residual_scale), eps=float(eps),
-                          dtype=_DTYPES[x.dtype], post_kind=_NORMS[post_norm], norm_kind=_NORMS[norm])
-    kept = []
-    for name, t, vector in (("gate", gate, False), ("post_weight", post_weight, True), ("post_bias", post_bias, True),
-                            ("weight", weight, True), ("bias", bias, True), ("mod_scale", mod_scale, False),
-                            ("mod_shift", mod_shift, False)):
-        param, tensor = _param(t, x, rows, name, vector=vector)
-        setattr(args, name, param)
-        kept.append(tensor)
+    kept = []  # copies made for alignment live until the launch
+    gate, mod_scale, mod_shift = (_row_param(t, kept, rows, width, dtype, device, name) for t, name in (
+        (gate, "gate"), (mod_scale, "mod_scale"), (mod_shift, "mod_shift")))
+    post_weight, post_bias, weight, bias = (_channel_param(t, kept, width, dtype, device, name) for t, name in (
+        (post_weight, "post_weight"), (post_bias, "post_bias"), (weight, "weight"), (bias, "bias")))
     h, z = x, None
+    branch_ptr = h_ptr = z_ptr = scales_ptr = 0
     if branch is not None:
+        if branch.shape != shape or branch.dtype is not dtype or branch.device != device:
+            raise ValueError("branch must match x's shape, dtype and device.")
         branch = _vectors(branch)
-        h = _output(out, x.shape, x.dtype, x.device)
-        args.branch, args.h_out = branch.data_ptr(), h.data_ptr()
+        h = torch.empty_like(x_rows) if out is None else _checked_output(out, shape, dtype, device)
+        branch_ptr, h_ptr = branch.data_ptr(), h.data_ptr()
     if norm is not None:
-        z = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn if quantize else x.dtype)
-        args.z_out = z.data_ptr()
+        z = torch.empty_like(x_rows, dtype=_E4M3) if quantize else torch.empty_like(x_rows)
+        z_ptr = z.data_ptr()
         if quantize:
-            scales = _scales_for(rows, width, x.device)
-            args.scales, args.scales_row_stride, args.scales_group_stride = scales.data_ptr(), scales.stride(0), scales.stride(1)
+            scales = _scales_for(rows, width, device)
+            scales_ptr = scales.data_ptr()
             z = (z, scales)
-    if rows == 0:
-        return h, z
-    with torch.cuda.device(x.device):
-        status = _lib.load_library().sq_block_norm(_lib.ctypes.byref(args), _stream())
-    _lib.check(status, "sq_block_norm")
+    if rows:
+        _call("sq_block_norm", device,
+              _lib.BLOCK_NORM.pack(x_rows.data_ptr(), branch_ptr, *gate, *post_weight, *post_bias, *weight, *bias, *mod_scale,
+                                   *mod_shift, h_ptr, z_ptr, scales_ptr, 1, rows, rows, width, residual_scale, eps,
+                                   _DTYPES[dtype], _NORMS[post_norm], _NORMS[norm], 0))
     return h, z
 
 
+_NO_SECTIONS = (0,) * _lib.ROTARY_AXES
 _POSITIONS = {torch.int32: _lib.POS_INT32, torch.int64: _lib.POS_INT64, torch.float32: _lib.POS_FP32}
 _ROTARY_LAYOUTS = {"interleaved": _lib.ROTARY_INTERLEAVED, "half": _lib.ROTARY_HALF}
 _ROTARY_NORMS = {None: _lib.ROTARY_NORM_NONE, "head": _lib.ROTARY_NORM_HEAD, "token": _lib.ROTARY_NORM_TOKEN}
 
 
-def _heads_view(t: torch.Tensor, name: str) -> torch.Tensor:
-    """[batch, tokens, heads, dim] with vectors the kernel can read in place, or a copy that has them."""
-    if t.stride(3) == 1 and all(s % 8 == 0 for s in t.stride()[:3]) and t.data_ptr() % 16 == 0:
-        return t
-    return _vectors(t)
+def _heads_input(t: torch.Tensor):
+    """(tensor, pointer, batch / token / head strides) with vectors the kernel can read in place, or a copy that has them."""
+    b, s, h, d = t.stride()
+    pointer = t.data_ptr()
+    if d != 1 or (b | s | h) % 8 or pointer % 16:
+        t = _vectors(t)
+        b, s, h, d = t.stride()
+        pointer = t.data_ptr()
+    return t, pointer, (b, s, h)
 
 
-def _heads_output(out, like: torch.Tensor, name: str) -> torch.Tensor:
+def _heads_output(out, like, shape, dtype, device, name: str):
     if out is None:
-        return torch.empty(like.shape, device=like.device, dtype=like.dtype)
-    fits = (out.shape == like.shape and out.dtype == like.dtype and out.device == like.device and out.stride(3) == 1
-            and all(s % 8 == 0 and (s > 0 or n == 1) for s, n in zip(out.stride()[:3], out.shape)) and out.data_ptr() % 16 == 0)
+        out = like.new_empty(shape)
+        return out, out.data_ptr(), (shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3])
+    strides = out.stride()
+    fits = (out.shape == shape and out.dtype is dtype and out.device == device and strides[3] == 1 and out.data_ptr() % 16 == 0
+            and all(s % 8 == 0 and (s > 0 or n == 1) for s, n in zip(strides[:3], shape)))
     if not fits:
         raise ValueError(f"out for {name} must match it, with a contiguous last axis, strides that are multiples of 8 "
                          "elements and 16-byte alignment.")
-    return out
+    return out, out.data_ptr(), strides[:3]
+
+
+def _rotary_weight(t, kept: list, count: int, dim: int, norm, dtype, device, name: str):
+    if t is None:
+        return 0, False
+    if norm is None:
+        raise ValueError("q_weight and k_weight belong to a norm.")
+    f32 = t.dtype is torch.float32
+    if t.device != device or not (f32 or t.dtype is dtype) or t.shape != ((count * dim,) if norm == "token" else (dim,)):
+        raise ValueError(f"{name} must be [dim] (head norm) or [heads * dim] (token norm), in q's dtype or float32, on its device.")
+    pointer = t.data_ptr()
+    if pointer % 16 or not t.is_contiguous():
+        t = _vectors(t)
+        kept.append(t)
+        pointer = t.data_ptr()
+    return pointer, f32
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, *, sections,
@@ -514,68 +567,59 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     int64 or float32, any value, however far or negative: angles are reduced in 64 bits (the rotation by
     ``-positions`` undoes it).  ``layout``: pairs are neighbours ("interleaved") or half the rotated length apart
     ("half"); elements past 2 * pairs pass through.  ``norm``: RMS of each head ("head", weights [dim]) or over all
-    heads of a token ("token", weights [heads * dim]).  ``out`` is a pair (q, k) of tensors to write, strided as a
-    cache or a transposed view may be; they may be the inputs themselves, but overlap nothing otherwise."""
-    for t, name in ((q, "q"), (k, "k")):
-        if t is None and name == "k":
-            continue
-        _require_cuda(t, name)
-        if t.ndim != 4 or t.dtype not in _DTYPES:
-            raise ValueError(f"{name} must be a bf16 or fp16 tensor [batch, tokens, heads, dim].")
+    heads of a token ("token", weights [heads * dim]), statistics in fp32 (values up to 2^59).  ``out`` is a pair (q, k) of
+    tensors to write, strided as a cache or a transposed view may be; they may be the inputs themselves, but overlap
+    nothing otherwise."""
+    if not q.is_cuda:
+        _require_cuda(q, "q")
+    if q.ndim != 4 or q.dtype not in _DTYPES:
+        raise ValueError("q must be a bf16 or fp16 tensor [batch, tokens, heads, dim].")
     out_q, out_k = out if out is not None else (None, None)
     _no_gradient(q, k, q_weight, k_weight, inv_freq, positions, out_q, out_k)
-    batch, tokens, heads, dim = q.shape
-    if k is not None and (k.dtype != q.dtype or k.device != q.device or (k.shape[0], k.shape[1], k.shape[3]) != (batch, tokens, dim)):
-        raise ValueError("k must match q in dtype, device, batch, tokens and dim.")
-    if k is None and (k_weight is not None or out_k is not None):
+    device, shape, dtype = q.device, q.shape, q.dtype
+    batch, tokens, heads, dim = shape
+    kv_heads = 0
+    if k is not None:
+        k_shape = k.shape
+        if k.ndim != 4 or k.dtype is not dtype or k.device != device or (k_shape[0], k_shape[1], k_shape[3]) != (batch, tokens, dim):
+            raise ValueError("k must match q in dtype, device, batch, tokens and dim.")
+        kv_heads = k_shape[2]
+    elif k_weight is not None or out_k is not None:
         raise ValueError("there is no k to weigh or to write.")
-    kv_heads = 0 if k is None else k.shape[2]
-    sections = tuple(int(s) for s in sections)
-    pairs = sum(sections)
-    if not 1 <= len(sections) <= _lib.ROTARY_AXES or min(sections) < 0 or pairs < 1 or 2 * pairs > dim:
+    axes, pairs = len(sections), sum(sections)
+    if not 1 <= axes <= _lib.ROTARY_AXES or min(sections) < 0 or pairs < 1 or 2 * pairs > dim:
         raise ValueError(f"sections must be the pairs of 1 to {_lib.ROTARY_AXES} axes, at most dim / 2 together.")
-    lanes = 1 << max(dim // 8 - 1, 0).bit_length()
+    lanes = 1 << (dim // 8 - 1).bit_length() if dim >= 8 else 0
     if dim % 8 or not 8 <= dim <= 256 or heads == 0 or (k is not None and kv_heads == 0) or (heads + kv_heads) * lanes > 4096:
         raise ValueError(f"Unsupported head shape: {heads} + {kv_heads} heads of {dim}.")
     if layout not in _ROTARY_LAYOUTS or norm not in _ROTARY_NORMS:
         raise ValueError("layout must be 'interleaved' or 'half', norm None, 'head' or 'token'.")
-    if norm is None and (q_weight is not None or k_weight is not None):
-        raise ValueError("q_weight and k_weight belong to a norm.")
-    _on_device(q, positions=positions, inv_freq=inv_freq, q_weight=q_weight, k_weight=k_weight)
-    if inv_freq.dtype != torch.float64 or inv_freq.shape != (pairs,) or not inv_freq.is_contiguous():
-        raise ValueError("inv_freq must be contiguous float64 [pairs].")
-    if (positions.dtype not in _POSITIONS or positions.ndim not in (2, 3) or positions.shape[-2:] != (tokens, len(sections))
-            or (positions.ndim == 3 and positions.shape[0] not in (1, batch))):
-        raise ValueError("positions must be int32, int64 or float32 [tokens, axes] or [batch, tokens, axes].")
+    if inv_freq.dtype is not torch.float64 or inv_freq.shape != (pairs,) or not inv_freq.is_contiguous() or inv_freq.device != device:
+        raise ValueError("inv_freq must be contiguous float64 [pairs] on the input's device.")
+    p_shape = positions.shape
+    if (positions.dtype not in _POSITIONS or len(p_shape) not in (2, 3) or p_shape[-2:] != (tokens, axes)
+            or (len(p_shape) == 3 and p_shape[0] not in (1, batch)) or positions.device != device):
+        raise ValueError("positions must be int32, int64 or float32 [tokens, axes] or [batch, tokens, axes] on the input's device.")
     if positions.stride(-1) != 1:
         positions = positions.contiguous()
-    weights = []
-    for t, name, count in ((q_weight, "q_weight", heads), (k_weight, "k_weight", kv_heads)):
-        if t is not None:
-            if t.dtype not in (q.dtype, torch.float32) or t.shape != ((count * dim,) if norm == "token" else (dim,)):
-                raise ValueError(f"{name} must be [dim] (head norm) or [heads * dim] (token norm), in q's dtype or float32.")
-            t = _vectors(t)
-        weights.append(t)
-    q_in, k_in = _heads_view(q, "q"), None if k is None else _heads_view(k, "k")
-    q_out = _heads_output(out_q, q, "q")
-    k_out = None if k is None else _heads_output(out_k, k, "k")
-    if batch * tokens == 0:
-        return q_out, k_out
-    three = lambda t: (0, 0, 0) if t is None else t.stride()[:3]
-    args = _lib.Rotary(q=q_in.data_ptr(), k=_ptr(k_in), q_out=q_out.data_ptr(), k_out=_ptr(k_out),
-                       q_weight=_ptr(weights[0]), k_weight=_ptr(weights[1]), positions=positions.data_ptr(),
-                       position_batch_stride=positions.stride(0) if positions.ndim == 3 and positions.shape[0] > 1 else 0,
-                       position_token_stride=positions.stride(-2), inv_freq=inv_freq.data_ptr(), batch=batch, length=tokens,
-                       heads=heads, kv_heads=kv_heads, dim=dim, axes=len(sections), dtype=_DTYPES[q.dtype],
-                       layout=_ROTARY_LAYOUTS[layout], norm=_ROTARY_NORMS[norm], position_type=_POSITIONS[positions.dtype],
-                       q_weight_fp32=int(weights[0] is not None and weights[0].dtype == torch.float32),
-                       k_weight_fp32=int(weights[1] is not None and weights[1].dtype == torch.float32), eps=float(eps))
-    args.q_strides[:], args.k_strides[:] = three(q_in), three(k_in)
-    args.q_out_strides[:], args.k_out_strides[:] = three(q_out), three(k_out)
-    args.sections[:len(sections)] = sections
-    with torch.cuda.device(q.device):
-        status = _lib.load_library().sq_rotary(_lib.ctypes.byref(args), _stream())
-    _lib.check(status, "sq_rotary")
+    p_strides = positions.stride()
+    kept = []  # copies made for alignment live until the launch
+    q_weight, q_f32 = _rotary_weight(q_weight, kept, heads, dim, norm, dtype, device, "q_weight")
+    k_weight, k_f32 = _rotary_weight(k_weight, kept, kv_heads, dim, norm, dtype, device, "k_weight")
+    q, q_ptr, q_strides = _heads_input(q)
+    q_out, q_to, q_out_strides = _heads_output(out_q, q, shape, dtype, device, "q")
+    k_out, k_ptr, k_to = None, 0, 0
+    k_strides = k_out_strides = (0, 0, 0)
+    if k is not None:
+        k, k_ptr, k_strides = _heads_input(k)
+        k_out, k_to, k_out_strides = _heads_output(out_k, k, k_shape, dtype, device, "k")
+    if batch * tokens:
+        _call("sq_rotary", device,
+              _lib.ROTARY.pack(q_ptr, k_ptr, q_to, k_to, *q_strides, *k_strides, *q_out_strides, *k_out_strides, q_weight, k_weight,
+                               positions.data_ptr(), p_strides[0] if len(p_shape) == 3 and p_shape[0] > 1 else 0, p_strides[-2],
+                               inv_freq.data_ptr(), batch, tokens, heads, kv_heads, dim, axes, *sections, *_NO_SECTIONS[axes:],
+                               _DTYPES[dtype], _ROTARY_LAYOUTS[layout], _ROTARY_NORMS[norm], _POSITIONS[positions.dtype],
+                               q_f32, k_f32, eps, 0))
     return q_out, k_out
 
 
