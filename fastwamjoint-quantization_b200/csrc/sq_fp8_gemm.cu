@@ -17,6 +17,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <cstdlib>
 #include <mutex>
 
 #include "sq_internal.h"
@@ -87,6 +88,17 @@ __device__ __forceinline__ float4 load_peer(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
+}
+
+// Hand an accumulator back to the MMA issuer: arrive without release.  What has to come first - the warp's tensor-memory
+// loads - has completed (tcgen05.wait::ld, values in registers).  A releasing arrive would also wait for the thread's
+// outstanding global loads, the scales requested two runs ahead: 1000 to 1600 cycles in every run of 128 k (measured,
+// 893 us instead of 469 for 8192 x 14336 x 4096).
+__device__ __forceinline__ void mbar_arrive_relaxed(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_peer_relaxed(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 
 __device__ __forceinline__ void report_timeout(int* status, volatile int* abort_flag, int code) {
@@ -276,7 +288,7 @@ __global__ void __launch_bounds__(128 + 32 * few_drain_warps(TOK), 1)
       tmem_ld_chunk(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * TOK + share * kCols, d);
       tmem_wait_ld_of(d);
       tc_fence_before_sync();
-      if (lane == 0) mbar_arrive(bar_acc_empty + 8 * acc);
+      if (lane == 0) mbar_arrive_relaxed(bar_acc_empty + 8 * acc);
 #pragma unroll
       for (int i = 0; i < kCols / 4; ++i) {
         const float4 f = *reinterpret_cast<const float4*>(mine + 4 * i);
@@ -337,6 +349,406 @@ __global__ void __launch_bounds__(128 + 32 * few_drain_warps(TOK), 1)
   if (parts > 1) cluster_sync();  // the others may still be reading this thread block's sums
 }
 
+// ---------------------------------------------------------------------------------------------- many tokens
+constexpr int kPairTokens = 256;  // of a tile: 128 per thread block of the pair
+constexpr int kPairThreads = 384;
+constexpr int kFactorSlots = 8;
+constexpr uint32_t kFactorBytes = 2 * 128 * 4;  // the factors of a run: 128 tokens for each half of the channels
+constexpr int kStoreBoxes = 3;
+constexpr uint32_t kStoreBytes = 32 * 32 * 2;   // a drain warp's output box: 32 tokens x 32 channels
+__host__ __device__ constexpr int pair_stages(int bn) { return bn == 256 ? 5 : 7; }
+__host__ __device__ constexpr uint32_t pair_stage_bytes(int bn) { return kRun * kRun + bn / 2 * kRun; }
+__host__ __device__ constexpr uint32_t pair_smem(int bn) {
+  return pair_stages(bn) * pair_stage_bytes(bn) + 8 * kStoreBoxes * kStoreBytes + kFactorSlots * kFactorBytes + 512 + 1024;
+}
+
+__device__ __forceinline__ void umma_f8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+      "}\n"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// arrive once on the barrier at this offset in both thread blocks when the MMAs issued so far are done
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t dst_smem, uint32_t columns) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(columns) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t columns) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(columns) : "memory");
+}
+// box -> this thread block's shared memory, completion on a barrier of the pair's first thread block
+__device__ __forceinline__ void tma_load_pair(uint32_t dst_smem, const void* tmap, int32_t x, int32_t y, uint32_t leader_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(leader_bar)
+      : "memory");
+}
+
+// A pair of thread blocks (cluster of two, tcgen05 cta_group::2) owns tiles of 256 tokens x BN channels: each loads its 128
+// tokens and half of the channels, the tensor cores of both read both halves of the weights, and each drains its own
+// 128 tokens.  A weight tile thus crosses shared memory half as often per product as with one thread block per tile,
+// whose operand reads would fill the shared-memory bandwidth.
+//
+// Drain: lane = token, so the run's factor is ONE number per thread (token scale x weight-block scale; a warp's channels
+// lie in one weight block) and an element costs one fma.  (Packed fmas made the compiler copy 90 registers per run into
+// aligned pairs: 558 us against 452 for 8192 x 14336 x 4096.)  The factors are made by a warp of their own, which
+// multiplies them into a ring in shared memory: loads and addresses in the drain loop cost more than the sums.
+// Tensor memory holds four accumulators of 128 columns.  With BN = 256 a run is two products of 128 channels, each with
+// an accumulator and four drain warps of its own, so that the tensor core has three more to work on while one is
+// drained and handed back.
+// Persistent: tiles are dealt out statically, loads and MMAs run ahead over tile ends, results leave through small
+// swizzled boxes per warp and TMA stores.
+template <int BN, typename OutT>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    sq_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_weight,
+                       const __grid_constant__ CUtensorMap map_out, const Fp8Args p) {
+  constexpr int S = pair_stages(BN);
+  constexpr int kParts = BN / 128;      // products of 128 channels in a run
+  constexpr int kDepth = 4 / kParts;    // runs whose accumulators fit tensor memory
+  constexpr int kCols = BN / 2;         // channels of a drain warp
+  // Batch b of four runs' factors takes the place of batch b - 2: it is written when the MMAs of run 4 b - 5 + kDepth are
+  // done, since these waited for the drain of run 4 b - 5, the last to read that place.  The next phase of the same
+  // barrier, S runs on, waits for the drain of run 4 b - 5 + S >= 4 b and so for this batch: it cannot pass unseen.  (Batch 1
+  // waits for run 2, whose next phase waits for the drain of run 2 + S - kDepth = 5.)
+  static_assert(S >= 5 && kFactorSlots == 8, "two batches of four runs");
+  constexpr uint32_t kXBytes = kRun * kRun, kWBytes = BN / 2 * kRun;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t x_ring = base, w_ring = base + S * kXBytes, store_ring = w_ring + S * kWBytes;
+  const uint32_t factors = store_ring + 8 * kStoreBoxes * kStoreBytes;
+  const uint32_t bars = factors + kFactorSlots * kFactorBytes;
+  const uint32_t bar_full = bars, bar_empty = bars + 8 * S, bar_acc_full = bars + 16 * S, bar_acc_empty = bar_acc_full + 32;
+  const uint32_t bar_factor = bar_acc_empty + 32;
+  const uint32_t words = bar_factor + 16;
+  volatile uint32_t* tmem_word = reinterpret_cast<volatile uint32_t*>(gen + (words - base));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + (words + 4 - base));
+  volatile int* keep_on = reinterpret_cast<volatile int*>(gen + (words + 8 - base));  // an abort flag that nobody sets
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, kParts);
+    }
+    for (int b = 0; b < 4; ++b) {
+      mbar_init(bar_acc_full + 8 * b, 1);
+      mbar_init(bar_acc_empty + 8 * b, 16 / kParts);  // the accumulator's drain warps of both thread blocks
+    }
+    for (int i = 0; i < 2; ++i) mbar_init(bar_factor + 8 * i, 1);
+    *abort_flag = 0;
+    *keep_on = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&map_codes);
+    tma_prefetch_desc(&map_weight);
+    tma_prefetch_desc(&map_out);
+  }
+  if (warp == 2) tmem_alloc_pair(words, 512);
+  __syncwarp();
+  tc_fence_before_sync();
+  cluster_sync();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_word;
+
+  const int tiles = p.ch_tiles * p.tok_tiles, pairs = static_cast<int>(gridDim.x >> 1);
+  const int first = static_cast<int>(blockIdx.x >> 1);
+  // tiles in strips of 8 token tiles, channels along the strip: what runs at one time shares tokens and weights in L2
+  auto place = [&](int tile, int64_t& tok, int& ch) {
+    const int strip = tile / (8 * p.ch_tiles), left = tile - strip * 8 * p.ch_tiles;
+    const int height = min(8, p.tok_tiles - strip * 8);
+    const int column = left / height;
+    tok = static_cast<int64_t>(strip * 8 + left - column * height) * kPairTokens + rank * 128;
+    ch = column * BN;
+  };
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0) {
+      // TMA producer.  Each thread block loads its own tokens and, of every product's 128 channels, 64.
+      uint32_t s = 0, phase = 0, issued = 0;
+      const int ahead = first < tiles ? min(S, p.runs) : 0;
+      int64_t tok = 0;
+      int ch = 0;
+      auto load_weights = [&](uint32_t stage, int g) {
+        const uint32_t bar = peer_address(bar_full + 8 * stage, 0);
+        if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * stage, 2 * (kXBytes + kWBytes));
+#pragma unroll
+        for (int h = 0; h < kParts; ++h)
+          tma_load_pair(w_ring + stage * kWBytes + h * 64 * kRun, &map_weight, g * kRun, ch + h * 128 + static_cast<int>(rank) * 64, bar);
+      };
+      auto load_codes = [&](uint32_t stage, int g) {
+        tma_load_pair(x_ring + stage * kXBytes, &map_codes, g * kRun, static_cast<int32_t>(tok), peer_address(bar_full + 8 * stage, 0));
+      };
+      if (ahead > 0) {
+        // the first weights do not come from the kernel in front: requested before waiting for it
+        place(first, tok, ch);
+        if (elect_one()) {
+          for (int i = 0; i < ahead; ++i) load_weights(i, i);
+        }
+        __syncwarp();
+      }
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      if (ahead > 0) {
+        if (elect_one()) {
+          for (int i = 0; i < ahead; ++i) load_codes(i, i);
+        }
+        __syncwarp();
+        issued = ahead;
+        s = ahead == S ? 0 : ahead;
+        phase = ahead == S ? 1 : 0;
+      }
+      bool ok = true;
+      for (int tile = first; tile < tiles && ok; tile += pairs) {
+        place(tile, tok, ch);
+        for (int g = tile == first ? ahead : 0; g < p.runs; ++g, ++issued) {
+          if (!mbar_wait_bounded(bar_empty + 8 * s, phase ^ 1u, abort_flag, kWaitLimitNs)) {
+            if (lane == 0) report_timeout(p.status, abort_flag, 9211);
+            ok = false;
+            break;
+          }
+          if (elect_one()) {
+            load_weights(s, g);
+            load_codes(s, g);
+          }
+          __syncwarp();
+          if (++s == S) {
+            s = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // no copy may be in flight when the thread block leaves; the first one's barriers count both halves.  After a wait
+      // that ran out in the second one alone there is no barrier to ask: its copies take microseconds, it waits a second.
+      if (rank == 0) {
+        for (uint32_t i = issued > S ? issued - S : 0; i < issued; ++i)
+          mbar_wait_bounded(bar_full + 8 * (i % S), (i / S) & 1u, keep_on, kWaitLimitNs);
+      } else if (!ok) {
+        const uint64_t start = global_timer_ns();
+        while (global_timer_ns() - start < kWaitLimitNs) asm volatile("nanosleep.u32 1000;");
+      }
+    } else if (warp != 2 && rank == 0) {
+      // MMA issuers, for both thread blocks: two warps take the products of 128 channels in turn.  A product's two waits
+      // and the issue take a warp about 500 cycles beside the drain warps on its scheduler, twice what the tensor core
+      // takes for it.
+      constexpr uint32_t idesc = umma_idesc_e4m3(256, 128);
+      const uint32_t mine = warp >> 1;
+      uint32_t s = kParts == 2 ? 0 : mine, phase = 0, acc = mine, acc_phase = 0;
+      const uint64_t a0 = umma_desc_k128(x_ring), b0 = umma_desc_k128(w_ring + (kParts == 2 ? mine * 64 * kRun : 0));
+      const int my_tiles = first < tiles ? (tiles - first + pairs - 1) / pairs : 0;
+      const int64_t products = static_cast<int64_t>(my_tiles) * p.runs * kParts;
+      int64_t at = mine;
+      for (; at < products; at += 2) {
+        if (!mbar_wait_bounded(bar_full + 8 * s, phase, abort_flag, kWaitLimitNs)) {
+          if (lane == 0) report_timeout(p.status, abort_flag, 9213);
+          break;
+        }
+        if (!mbar_wait_bounded(bar_acc_empty + 8 * acc, acc_phase ^ 1u, abort_flag, kWaitLimitNs)) {
+          if (lane == 0) report_timeout(p.status, abort_flag, 9212);
+          break;
+        }
+        tc_fence_after_sync();
+        if (elect_one()) {
+          const uint64_t a = a0 + s * (kXBytes >> 4), b = b0 + s * (kWBytes >> 4);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) umma_f8_pair(tmem + acc * 128, a + 2 * i, b + 2 * i, idesc, i != 0);
+          umma_commit_pair(bar_acc_full + 8 * acc);
+          umma_commit_pair(bar_empty + 8 * s);
+        }
+        __syncwarp();
+        s += kParts == 2 ? 1 : 2;
+        if (s >= S) {
+          s -= S;
+          phase ^= 1u;
+        }
+        acc ^= 2;
+        acc_phase ^= acc == mine ? 1u : 0u;
+      }
+      // the accumulators still being written when a wait ran out: let the instructions end before the memory is freed
+      for (int64_t i = at >= 4 ? at - 4 : mine; i < at; i += 2)
+        mbar_wait_bounded(bar_acc_full + 8 * (i % 4), static_cast<uint32_t>(i / 4) & 1u, keep_on, kWaitLimitNs);
+    } else if (warp == 2) {
+      // Factors: four tokens and both halves' weight blocks per lane and run, in batches of four runs with one barrier each
+      // (a drain warp waits for factors every fourth run).  The arrive releases the stores and waits for whatever loads
+      // are under way: none, between the batches.
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      const int64_t rows32 = 32 * p.scales_row;
+      int tile = first, g = 0, rows = 0;
+      const float* token = nullptr;
+      const float* block[2] = {nullptr, nullptr};
+      auto aim = [&]() {
+        int64_t tok;
+        int ch;
+        place(tile, tok, ch);
+        rows = static_cast<int>(min(static_cast<int64_t>(128), p.M - tok)) - lane;  // of them 32 i < rows are there
+        token = p.scales + (rows > 0 ? tok + lane : 0) * p.scales_row;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int n = ch + h * kCols;
+          block[h] = p.weight_scales + static_cast<int64_t>(n < p.N ? n / kRun : 0) * p.runs;
+        }
+      };
+      if (first < tiles) aim();
+      static_assert(3 + kDepth == S, "the first run waited for is the second round of stage 0");
+      uint32_t batch = 0, s = 0, phase = 1;
+      for (; tile < tiles; ++batch) {
+        float t[4][4], w[4][2];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const bool in = tile < tiles;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) t[r][i] = in && 32 * i < rows ? __ldg(token + i * rows32) : 0.0f;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) w[r][h] = in ? __ldg(block[h] + g) : 0.0f;
+          token += p.scales_group;
+          if (in && ++g == p.runs) {
+            g = 0;
+            tile += pairs;
+            if (tile < tiles) aim();
+          }
+        }
+        if (batch == 1) {
+          // nothing is overwritten yet, but a phase is told from its neighbours by parity alone: run 2 done means that the
+          // first round of stage 0 has passed when its second one is waited for next
+          if (!mbar_wait_bounded(bar_empty + 16, 0, abort_flag, kWaitLimitNs)) {
+            if (lane == 0) report_timeout(p.status, abort_flag, 9215);
+            break;
+          }
+        } else if (batch >= 2) {
+          if (!mbar_wait_bounded(bar_empty + 8 * s, phase, abort_flag, kWaitLimitNs)) {
+            if (lane == 0) report_timeout(p.status, abort_flag, 9215);
+            break;
+          }
+          s += 4;
+          if (s >= S) {
+            s -= S;
+            phase ^= 1u;
+          }
+        }
+        const uint32_t to = factors + (batch & 1u) * 4 * kFactorBytes + lane * 4;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + r * kFactorBytes + h * 512 + i * 128), "f"(t[r][i] * w[r][h]) : "memory");
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_factor + 8 * (batch & 1u));
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    const int quarter = warp & 3, share = (warp - 4) >> 2;
+    const uint32_t store = store_ring + (warp - 4) * kStoreBoxes * kStoreBytes;
+    const uint32_t acc_empty = peer_address(bar_acc_empty, 0);
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (kParts == 1 ? share * kCols : 0);
+    const uint32_t my_factors = factors + share * 512 + (quarter * 32 + lane) * 4;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the results may overwrite what the kernel in front reads
+    uint32_t acc = kParts == 1 ? 0 : share, acc_phase = 0, run = 0, box = 0;
+    bool ready = false;  // the accumulator at hand was seen full while the last one was worked on
+    for (int tile = first; tile < tiles; tile += pairs) {
+      float sums[kCols];
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) sums[i] = 0.0f;
+      for (int g = 0; g < p.runs; ++g, ++run) {
+        uint32_t d[2][32];
+        float f;
+        if (!ready && !mbar_wait_bounded(bar_acc_full + 8 * acc, acc_phase, abort_flag, kWaitLimitNs)) {
+          if (lane == 0) report_timeout(p.status, abort_flag, 9214);
+          goto out;
+        }
+        __syncwarp();
+        tc_fence_after_sync();
+        const uint32_t from = lanes + acc * 128;
+        tmem_ld_32x32b_x32(from, d[0]);
+        if ((run & 3u) == 0 && !mbar_wait_bounded(bar_factor + ((run << 1) & 8u), (run >> 3) & 1u, abort_flag, kWaitLimitNs)) {
+          if (lane == 0) report_timeout(p.status, abort_flag, 9216);
+          goto out;
+        }
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(my_factors + (run & 7u) * kFactorBytes) : "memory");
+#pragma unroll
+        for (int c = 0; c < kCols / 32; ++c) {
+          tmem_wait_ld_of(d[c & 1]);
+          if (c + 1 < kCols / 32) {
+            tmem_ld_32x32b_x32(from + 32 * (c + 1), d[(c + 1) & 1]);
+          } else {
+            tc_fence_before_sync();
+            if (lane == 0) mbar_arrive_peer_relaxed(acc_empty + 8 * acc);
+            acc += kParts;
+            if (acc >= 4) {
+              acc -= 4;
+              acc_phase ^= 1u;
+            }
+            ready = mbar_test_wait(bar_acc_full + 8 * acc, acc_phase);
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sums[32 * c + i] = fmaf(__uint_as_float(d[c & 1][i]), f, sums[32 * c + i]);
+        }
+      }
+      int64_t tok;
+      int ch;
+      place(tile, tok, ch);
+      const int64_t row0 = tok + quarter * 32;
+      const int n0 = ch + share * kCols;
+      // 32 channels at a time: bias, rounding, a box of 32 x 32, out by TMA (it clips what lies outside).  The box is
+      // written again kStoreBoxes stores later.
+#pragma unroll
+      for (int part = 0; part < kCols / 32; ++part) {
+        const int n = n0 + part * 32;
+        uint4 packed[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = sums[part * 32 + c * 8 + e];
+          if (p.bias != nullptr && n + c * 8 < p.N) {
+            float b[8];
+            load_bias8<OutT>(p.bias, n + c * 8, b);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] += b[e];
+          }
+          packed[c] = pack8(y, static_cast<const OutT*>(nullptr));
+        }
+        if (lane == 0) tma_store_wait_read<kStoreBoxes - 1>();
+        __syncwarp();
+        const uint32_t to = store + box * kStoreBytes;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)  // 64-byte swizzle: 16-byte chunk c of row r at c ^ (r / 2 mod 4)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                       ::"r"(to + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)), "r"(packed[c].x), "r"(packed[c].y),
+                         "r"(packed[c].z), "r"(packed[c].w) : "memory");
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (n < p.N && row0 < p.M) tma_store_2d(&map_out, n, static_cast<int32_t>(row0), to);
+          tma_store_commit();  // an empty group where there is nothing to store: the count of groups stays the boxes'
+        }
+        box = box + 1 == kStoreBoxes ? 0 : box + 1;
+      }
+    }
+  out:
+    if (lane == 0) tma_store_wait<0>();
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  cluster_sync();
+  if (warp == 2) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
 // ---------------------------------------------------------------------------------------------- host side
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -365,6 +777,19 @@ bool make_map(CUtensorMap* map, const void* data, uint64_t rows, uint64_t row_by
   const cuuint32_t elem[2] = {1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(data), dims, strides, box, elem,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// [rows, n] of 16-bit results in boxes of [32, 32], 64-byte swizzle: what a drain warp stores
+bool make_store_map(CUtensorMap* map, void* data, int dtype, uint64_t rows, uint64_t n) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[2] = {n, rows};
+  const cuuint64_t strides[1] = {n * 2};
+  const cuuint32_t box[2] = {32, 32};
+  const cuuint32_t elem[2] = {1, 1};
+  return fn(map, dtype == SQ_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, data, dims, strides,
+            box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -417,6 +842,38 @@ int launch_few(const Fp8GemmArgs& a, Fp8Args p, int parts, cudaStream_t stream) 
   return err == cudaSuccess ? SQ_OK : static_cast<int>(err);
 }
 
+template <int BN, typename OutT>
+int launch_pair(const Fp8GemmArgs& a, Fp8Args p, cudaStream_t stream) {
+  auto kernel = sq_fp8_pair_kernel<BN, OutT>;
+  static bool configured[64] = {false};
+  const int ready = allow_smem(kernel, pair_smem(BN), configured);
+  if (ready != SQ_OK) return ready;
+  CUtensorMap map_codes, map_weight, map_out;
+  if (!make_map(&map_codes, a.codes, a.M, a.K, 128) || !make_map(&map_weight, a.weight, a.N, a.K, 64) ||
+      !make_store_map(&map_out, a.out, a.out_dtype, a.M, a.N))
+    return SQ_ERR_DRIVER;
+  p.ch_tiles = static_cast<int>((a.N + BN - 1) / BN);
+  p.tok_tiles = static_cast<int>((a.M + kPairTokens - 1) / kPairTokens);
+  const int64_t tiles = static_cast<int64_t>(p.ch_tiles) * p.tok_tiles;
+  if (tiles > 0x3FFFFFFF) return SQ_ERR_SHAPE;
+  const int64_t pairs = tiles < sm_count() / 2 ? tiles : sm_count() / 2;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(2 * pairs));
+  config.blockDim = dim3(kPairThreads);
+  config.dynamicSmemBytes = pair_smem(BN);
+  config.stream = stream;
+  cudaLaunchAttribute attribute[2];
+  attribute[0].id = cudaLaunchAttributeClusterDimension;
+  attribute[0].val.clusterDim.x = 2;
+  attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
+  attribute[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attribute;
+  config.numAttrs = a.after_quantize ? 2 : 1;
+  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, map_codes, map_weight, map_out, p);
+  return err == cudaSuccess ? SQ_OK : static_cast<int>(err);
+}
+
 // Thread blocks that share a tile's K: as many as keep the GPU in one wave, at most 8 (the portable cluster size).
 int pick_parts(int64_t tiles, int runs, int sms) {
   int parts = 1;
@@ -426,6 +883,10 @@ int pick_parts(int64_t tiles, int runs, int sms) {
 
 template <typename OutT>
 int launch_typed(const Fp8GemmArgs& a, const Fp8Args& p, cudaStream_t stream) {
+  static const int form = [] { const char* v = std::getenv("SQ_FP8_FORM"); return v ? std::atoi(v) : 0; }();
+  if (form == 256) return launch_pair<256, OutT>(a, p, stream);
+  if (form == 128) return launch_pair<128, OutT>(a, p, stream);
+  if (form == 0 && a.M >= 1024) return launch_pair<256, OutT>(a, p, stream);
   const int tok = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
   const int64_t tiles = static_cast<int64_t>(p.ch_tiles) * ((a.M + tok - 1) / tok);
   const int parts = pick_parts(tiles, p.runs, sm_count());
