@@ -17,7 +17,6 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
-#include <cstdlib>
 #include <mutex>
 
 #include "sq_internal.h"
@@ -814,6 +813,24 @@ int allow_smem(Kernel* kernel, uint32_t bytes, bool (&done)[64]) {
   return SQ_OK;
 }
 
+template <typename Kernel>
+cudaLaunchConfig_t cluster_config(Kernel*, int64_t blocks, int threads, uint32_t smem, int cluster, bool after_quantize,
+                                  cudaStream_t stream, cudaLaunchAttribute (&attribute)[2]) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(blocks));
+  config.blockDim = dim3(static_cast<unsigned>(threads));
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  attribute[0].id = cudaLaunchAttributeClusterDimension;
+  attribute[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
+  attribute[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attribute;
+  config.numAttrs = after_quantize ? 2 : 1;
+  return config;
+}
+
 template <int TOK, typename OutT>
 int launch_few(const Fp8GemmArgs& a, Fp8Args p, int parts, cudaStream_t stream) {
   auto kernel = sq_fp8_few_kernel<TOK, OutT>;
@@ -822,22 +839,13 @@ int launch_few(const Fp8GemmArgs& a, Fp8Args p, int parts, cudaStream_t stream) 
   if (ready != SQ_OK) return ready;
   CUtensorMap map_codes, map_weight;
   if (!make_map(&map_codes, a.codes, a.M, a.K, TOK) || !make_map(&map_weight, a.weight, a.N, a.K, kRun)) return SQ_ERR_DRIVER;
+  p.ch_tiles = static_cast<int>((a.N + kRun - 1) / kRun);
   p.tok_tiles = static_cast<int>((a.M + TOK - 1) / TOK);
   const int64_t blocks = static_cast<int64_t>(p.ch_tiles) * p.tok_tiles * parts;
   if (blocks > 0x7FFFFFFF) return SQ_ERR_SHAPE;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(blocks));
-  config.blockDim = dim3(128 + 32 * few_drain_warps(TOK));
-  config.dynamicSmemBytes = few_smem(TOK);
-  config.stream = stream;
   cudaLaunchAttribute attribute[2];
-  attribute[0].id = cudaLaunchAttributeClusterDimension;
-  attribute[0].val.clusterDim.x = static_cast<unsigned>(parts);
-  attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
-  attribute[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute[1].val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = attribute;
-  config.numAttrs = a.after_quantize ? 2 : 1;
+  const cudaLaunchConfig_t config = cluster_config(kernel, blocks, 128 + 32 * few_drain_warps(TOK), few_smem(TOK), parts,
+                                                   a.after_quantize, stream, attribute);
   const cudaError_t err = cudaLaunchKernelEx(&config, kernel, map_codes, map_weight, p);
   return err == cudaSuccess ? SQ_OK : static_cast<int>(err);
 }
@@ -855,47 +863,94 @@ int launch_pair(const Fp8GemmArgs& a, Fp8Args p, cudaStream_t stream) {
   p.ch_tiles = static_cast<int>((a.N + BN - 1) / BN);
   p.tok_tiles = static_cast<int>((a.M + kPairTokens - 1) / kPairTokens);
   const int64_t tiles = static_cast<int64_t>(p.ch_tiles) * p.tok_tiles;
-  if (tiles > 0x3FFFFFFF) return SQ_ERR_SHAPE;
+  if (tiles > 0x0FFFFFFF) return SQ_ERR_SHAPE;
   const int64_t pairs = tiles < sm_count() / 2 ? tiles : sm_count() / 2;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(2 * pairs));
-  config.blockDim = dim3(kPairThreads);
-  config.dynamicSmemBytes = pair_smem(BN);
-  config.stream = stream;
   cudaLaunchAttribute attribute[2];
-  attribute[0].id = cudaLaunchAttributeClusterDimension;
-  attribute[0].val.clusterDim.x = 2;
-  attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
-  attribute[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute[1].val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = attribute;
-  config.numAttrs = a.after_quantize ? 2 : 1;
+  const cudaLaunchConfig_t config = cluster_config(kernel, 2 * pairs, kPairThreads, pair_smem(BN), 2, a.after_quantize, stream, attribute);
   const cudaError_t err = cudaLaunchKernelEx(&config, kernel, map_codes, map_weight, map_out, p);
   return err == cudaSuccess ? SQ_OK : static_cast<int>(err);
 }
 
-// Thread blocks that share a tile's K: as many as keep the GPU in one wave, at most 8 (the portable cluster size).
-int pick_parts(int64_t tiles, int runs, int sms) {
-  int parts = 1;
-  while (parts < 8 && tiles * (parts * 2) <= sms && runs >= parts * 2) parts *= 2;
-  return parts;
+// Clusters of `parts` thread blocks with one thread block per SM that run at one time: fewer than SMs / parts where a
+// GPC's SMs are no multiple of `parts` (24 clusters of 6 do not fit 148 SMs).  Asked once per device.
+int cluster_capacity(int parts) {
+  static int cached[64][9] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return sm_count() / parts;
+  int& n = cached[dev][parts];
+  if (n == 0) {
+    auto kernel = sq_fp8_few_kernel<128, __nv_bfloat16>;
+    static bool configured[64] = {false};
+    cudaLaunchAttribute attribute[2];
+    const cudaLaunchConfig_t config = cluster_config(kernel, parts, 128 + 32 * few_drain_warps(128), few_smem(128), parts, false,
+                                                     nullptr, attribute);
+    int found = 0;
+    if (allow_smem(kernel, few_smem(128), configured) != SQ_OK || cudaOccupancyMaxActiveClusters(&found, kernel, &config) != cudaSuccess ||
+        found <= 0) {
+      cudaGetLastError();  // not a failure of the product: take the plain quotient
+      found = sm_count() / parts;
+    }
+    n = found;
+  }
+  return n;
+}
+
+// Which kernel, tile and split: the one with the least predicted time, waves * (runs * c + e) + start, in microseconds.  The
+// constants were measured on a B200 (N x K from 1024 x 14336 to 14336 x 1024, M from 1 to 2048): a run of 128 k costs a
+// few-token tile of 16 / 32 / 64 / 128 tokens 0.26 / 0.27 / 0.315 / 0.42 us and a pair's tile of 256 tokens 0.235 us (128
+// channels) or 0.36 us (256); a few-token tile's end costs 0.013 us per token whole and 0.022 + 0.0035 parts split.
+// Predictions are within 15 % of the measured times; what they decide, with both sides measured: 128 tokens into 4096 x 1024 as
+// 64-token tiles in two parts 7.1 us, as one 128-token tile 8.8; 294 tokens into 1024 x 14336 as 64-token tiles in three parts
+// 19.4, as pairs 30.1; 1592 into 4096 x 4096 as pairs with 256 channels 33.8, with 128 37.1, as few-token tiles 56.7.
+struct Fp8Plan {
+  int tok;    // 0: a pair of thread blocks
+  int parts;  // few tokens: thread blocks per tile; pair: channels
+};
+
+Fp8Plan pick_plan(int64_t M, int64_t N, int runs) {
+  constexpr int kTok[4] = {16, 32, 64, 128};
+  constexpr double kRunCost[4] = {0.26, 0.27, 0.315, 0.42};
+  Fp8Plan best = {0, 256};
+  double least = 1e30;
+  for (int bn = 256; bn >= 128; bn -= 128) {
+    const int64_t tiles = ((N + bn - 1) / bn) * ((M + kPairTokens - 1) / kPairTokens);
+    const int64_t at_once = sm_count() / 2;
+    const double cost = 4.5 + static_cast<double>((tiles + at_once - 1) / at_once) * (bn == 256 ? 0.36 * runs + 1.2 : 0.235 * runs + 0.7);
+    if (cost < least) {
+      least = cost;
+      best = {0, bn};
+    }
+  }
+  const int64_t channels = (N + kRun - 1) / kRun;
+  for (int i = 0; i < 4; ++i) {
+    const int64_t tiles = channels * ((M + kTok[i] - 1) / kTok[i]);
+    for (int parts = 1; parts <= 8 && parts <= runs; ++parts) {
+      const int at_once = cluster_capacity(parts);
+      const double end = kTok[i] * (parts == 1 ? 0.013 : 0.022 + 0.0035 * parts);
+      const double cost = 3.8 + static_cast<double>((tiles + at_once - 1) / at_once) * (kRunCost[i] * ((runs + parts - 1) / parts) + end);
+      if (cost < least) {
+        least = cost;
+        best = {kTok[i], parts};
+      }
+      if (tiles > at_once) break;  // a split of tiles that fill the GPU only adds ends
+    }
+    if (kTok[i] >= M) break;
+  }
+  return best;
 }
 
 template <typename OutT>
 int launch_typed(const Fp8GemmArgs& a, const Fp8Args& p, cudaStream_t stream) {
-  static const int form = [] { const char* v = std::getenv("SQ_FP8_FORM"); return v ? std::atoi(v) : 0; }();
-  if (form == 256) return launch_pair<256, OutT>(a, p, stream);
-  if (form == 128) return launch_pair<128, OutT>(a, p, stream);
-  if (form == 0 && a.M >= 1024) return launch_pair<256, OutT>(a, p, stream);
-  const int tok = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
-  const int64_t tiles = static_cast<int64_t>(p.ch_tiles) * ((a.M + tok - 1) / tok);
-  const int parts = pick_parts(tiles, p.runs, sm_count());
-  switch (tok) {
-    case 16: return launch_few<16, OutT>(a, p, parts, stream);
-    case 32: return launch_few<32, OutT>(a, p, parts, stream);
-    case 64: return launch_few<64, OutT>(a, p, parts, stream);
-    default: return launch_few<128, OutT>(a, p, parts, stream);
+  const Fp8Plan plan = pick_plan(a.M, a.N, p.runs);
+  switch (plan.tok) {
+    case 16: return launch_few<16, OutT>(a, p, plan.parts, stream);
+    case 32: return launch_few<32, OutT>(a, p, plan.parts, stream);
+    case 64: return launch_few<64, OutT>(a, p, plan.parts, stream);
+    case 128: return launch_few<128, OutT>(a, p, plan.parts, stream);
+    default: break;
   }
+  return plan.parts == 256 ? launch_pair<256, OutT>(a, p, stream) : launch_pair<128, OutT>(a, p, stream);
 }
 
 }  // namespace
@@ -929,7 +984,6 @@ int launch_fp8_gemm(const Fp8GemmArgs& a, cudaStream_t stream) {
   p.M = a.M;
   p.N = static_cast<int>(a.N);
   p.runs = static_cast<int>((a.K + kRun - 1) / kRun);
-  p.ch_tiles = static_cast<int>((a.N + kRun - 1) / kRun);
   return a.out_dtype == SQ_BF16 ? launch_typed<__nv_bfloat16>(a, p, stream) : launch_typed<__half>(a, p, stream);
 }
 
