@@ -37,22 +37,28 @@ struct NormArgs {
   int width;
 };
 
-// Sum over the TPR threads of a row, the same value in each of them and the same order in every run.
-template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float* partial) {
+// Sum over the threads of a block, the same value in each of them and the same order in every run.  Two buffers in turn:
+// one barrier per sum (a buffer is written again two sums later, past the barrier of the sum between).
+struct RowSum {
+  float* partial;  // [2][32]
+  int warps;
+  int buffer;
+  __device__ __forceinline__ float operator()(float v) {
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-  if (TPR > 32) {
-    const int warp = threadIdx.x >> 5;
-    __syncthreads();  // the last sum's readers are done with `partial`
-    if ((threadIdx.x & 31) == 0) partial[warp] = v;
-    __syncthreads();
-    v = 0.0f;
+    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    if (warps > 1) {
+      float* mine = partial + buffer * 32;
+      buffer ^= 1;
+      const int lane = threadIdx.x & 31;
+      if (lane == 0) mine[threadIdx.x >> 5] = v;
+      __syncthreads();
+      v = lane < warps ? mine[lane] : 0.0f;
 #pragma unroll
-    for (int w = 0; w < TPR / 32; ++w) v += partial[w];
+      for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    }
+    return v;
   }
-  return v;
-}
+};
 
 template <int VPT>
 __device__ __forceinline__ float local_squares(const float (&v)[VPT][8]) {
@@ -66,9 +72,9 @@ __device__ __forceinline__ float local_squares(const float (&v)[VPT][8]) {
 }
 
 // v -> (v - mean) / sqrt(variance + eps) or v / sqrt(mean square + eps); slots without elements stay zero
-template <int TPR, int VPT>
+template <int VPT>
 __device__ __forceinline__ void standardise(float (&v)[VPT][8], const bool (&on)[VPT], int kind, float eps, float inv_width,
-                                            float* partial) {
+                                            RowSum& row_sum) {
   if (kind == SQ_NORM_LAYER) {
     float share = 0.0f;  // of the mean: added up as v / width, which cannot overflow
 #pragma unroll
@@ -76,14 +82,14 @@ __device__ __forceinline__ void standardise(float (&v)[VPT][8], const bool (&on)
 #pragma unroll
       for (int e = 0; e < 8; ++e) share = fmaf(v[i][e], inv_width, share);
     }
-    const float mean = row_sum<TPR>(share, partial);
+    const float mean = row_sum(share);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[i][e] = on[i] ? v[i][e] - mean : 0.0f;
     }
   }
-  float squares = row_sum<TPR>(local_squares(v), partial);
+  float squares = row_sum(local_squares(v));
   if (!(squares < __int_as_float(0x7F800000))) {
     // the squares of bf16 values beyond 2^59 or so overflow: the row over again, 2^70 times smaller (eps is nothing next
     // to such a row).  The sum is the same in every thread of the row, so all of them come here or none.
@@ -92,7 +98,7 @@ __device__ __forceinline__ void standardise(float (&v)[VPT][8], const bool (&on)
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[i][e] *= 8.470329472543003e-22f;
     }
-    squares = row_sum<TPR>(local_squares(v), partial);
+    squares = row_sum(local_squares(v));
     eps = 0.0f;
   }
   const float r = rsqrtf(fmaf(squares, inv_width, eps));
@@ -103,61 +109,49 @@ __device__ __forceinline__ void standardise(float (&v)[VPT][8], const bool (&on)
   }
 }
 
-// where a row's parameters start; computed once per row (a division)
-__device__ __forceinline__ int64_t param_base(const Param& q, int64_t row) {
-  return q.span > 0 ? static_cast<int64_t>(static_cast<uint32_t>(row) / q.span) * q.stride : 0;
-}
-template <typename T>
-__device__ __forceinline__ void params_at(const Param& q, int64_t base, int column, float (&v)[8]) {
-  load_params<T>(q.p, base + column, q.f32 != 0, v);
+// where a row's parameters start
+__device__ __forceinline__ int64_t param_base(const Param& q, uint32_t row) {
+  return q.span > 0 ? static_cast<int64_t>(row / q.span) * q.stride : 0;
 }
 
-// TPR threads cover a row, thread t owning the vectors t, t + TPR, ... (VPT of them): a warp reads 512 contiguous
-// bytes, and the 16 vectors of a run of 128 sit in 16 neighbouring lanes.
-template <typename T, int TPR, int VPT, bool kBranch>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) sq_block_norm_kernel(const NormArgs a) {
-  constexpr int kRowsPerBlock = TPR < 128 ? 128 / TPR : 1;
-  __shared__ float partial[TPR / 32];
-  const int t = threadIdx.x % TPR;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + threadIdx.x / TPR;
-  const bool row_on = row < a.rows;  // rows of a block past the last one: only where a warp is a row of its own
-  if (!row_on) return;
+// A block takes a row, thread t owning the vectors t and t + blockDim: a warp reads 512 contiguous bytes, and the 16 vectors
+// of a run of 128 sit in 16 neighbouring lanes.
+template <typename T, int VPT, bool kBranch, int kMaxThreads, int kMinBlocks>
+__global__ void __launch_bounds__(kMaxThreads, kMinBlocks) sq_block_norm_kernel(const NormArgs a) {
+  __shared__ float partial[64];
+  RowSum row_sum{partial, static_cast<int>(blockDim.x >> 5), 0};
   const T* tag = nullptr;
-  const int64_t base = row * a.width;
+  const uint32_t row = blockIdx.x;
+  const int64_t base = static_cast<int64_t>(row) * a.width;
+  int column[VPT];
   bool on[VPT];
-  uint4 raw_x[VPT], raw_b[kBranch ? VPT : 1];
+  uint4 raw_x[VPT], raw_b[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int column = (t + i * TPR) * 8;
-    on[i] = column < a.width;
-    raw_x[i] = on[i] ? load_stream(static_cast<const T*>(a.x) + base + column) : make_uint4(0, 0, 0, 0);
-  }
-  if (kBranch) {
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-      raw_b[i] = on[i] ? load_stream(static_cast<const T*>(a.branch) + base + (t + i * TPR) * 8) : make_uint4(0, 0, 0, 0);
+    column[i] = static_cast<int>(threadIdx.x + i * blockDim.x) * 8;
+    on[i] = column[i] < a.width;
+    raw_x[i] = on[i] ? load_stream(static_cast<const T*>(a.x) + base + column[i]) : make_uint4(0, 0, 0, 0);
+    if (kBranch) raw_b[i] = on[i] ? load_stream(static_cast<const T*>(a.branch) + base + column[i]) : make_uint4(0, 0, 0, 0);
   }
   const int64_t gate_base = kBranch ? param_base(a.gate, row) : 0;
   const int64_t scale_base = param_base(a.mod_scale, row), shift_base = param_base(a.mod_shift, row);
   const float inv_width = 1.0f / static_cast<float>(a.width);
-  float h[VPT][8];
-  float p[8];
+  float h[VPT][8], p[8];
   if (kBranch) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) unpack8(raw_b[i], h[i], tag);
     if (a.post_kind != SQ_NORM_NONE) {
-      standardise<TPR, VPT>(h, on, a.post_kind, a.eps, inv_width, partial);
+      standardise<VPT>(h, on, a.post_kind, a.eps, inv_width, row_sum);
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
-        const int column = (t + i * TPR) * 8;
         if (!on[i]) continue;
         if (a.post_weight.p != nullptr) {
-          params_at<T>(a.post_weight, 0, column, p);
+          load_params<T>(a.post_weight.p, column[i], a.post_weight.f32 != 0, p);
 #pragma unroll
           for (int e = 0; e < 8; ++e) h[i][e] *= p[e];
         }
         if (a.post_bias.p != nullptr) {
-          params_at<T>(a.post_bias, 0, column, p);
+          load_params<T>(a.post_bias.p, column[i], a.post_bias.f32 != 0, p);
 #pragma unroll
           for (int e = 0; e < 8; ++e) h[i][e] += p[e];
         }
@@ -165,9 +159,9 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) sq_block_norm_kernel(co
     }
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int column = (t + i * TPR) * 8;
-      if (on[i] && a.gate.p != nullptr) {
-        params_at<T>(a.gate, gate_base, column, p);
+      if (!on[i]) continue;
+      if (a.gate.p != nullptr) {
+        load_params<T>(a.gate.p, gate_base + column[i], a.gate.f32 != 0, p);
 #pragma unroll
         for (int e = 0; e < 8; ++e) h[i][e] *= p[e];
       }
@@ -175,76 +169,71 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) sq_block_norm_kernel(co
       unpack8(raw_x[i], xv, tag);
 #pragma unroll
       for (int e = 0; e < 8; ++e) h[i][e] = fmaf(a.residual_scale, xv[e], h[i][e]);
-      if (on[i]) *reinterpret_cast<uint4*>(static_cast<T*>(a.h_out) + base + column) = pack8(h[i], tag);
+      *reinterpret_cast<uint4*>(static_cast<T*>(a.h_out) + base + column[i]) = pack8(h[i], tag);
     }
     if (a.norm_kind == SQ_NORM_NONE) return;
   } else {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) unpack8(raw_x[i], h[i], tag);
   }
-  standardise<TPR, VPT>(h, on, a.norm_kind, a.eps, inv_width, partial);
+  standardise<VPT>(h, on, a.norm_kind, a.eps, inv_width, row_sum);
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int column = (t + i * TPR) * 8;
     if (on[i]) {
       if (a.weight.p != nullptr) {
-        params_at<T>(a.weight, 0, column, p);
+        load_params<T>(a.weight.p, column[i], a.weight.f32 != 0, p);
 #pragma unroll
         for (int e = 0; e < 8; ++e) h[i][e] *= p[e];
       }
       if (a.bias.p != nullptr) {
-        params_at<T>(a.bias, 0, column, p);
+        load_params<T>(a.bias.p, column[i], a.bias.f32 != 0, p);
 #pragma unroll
         for (int e = 0; e < 8; ++e) h[i][e] += p[e];
       }
       if (a.mod_scale.p != nullptr) {
-        params_at<T>(a.mod_scale, scale_base, column, p);
+        load_params<T>(a.mod_scale.p, scale_base + column[i], a.mod_scale.f32 != 0, p);
 #pragma unroll
         for (int e = 0; e < 8; ++e) h[i][e] = fmaf(h[i][e], p[e], h[i][e]);
       }
       if (a.mod_shift.p != nullptr) {
-        params_at<T>(a.mod_shift, shift_base, column, p);
+        load_params<T>(a.mod_shift.p, shift_base + column[i], a.mod_shift.f32 != 0, p);
 #pragma unroll
         for (int e = 0; e < 8; ++e) h[i][e] += p[e];
       }
-      if (a.scales == nullptr) *reinterpret_cast<uint4*>(static_cast<T*>(a.z_out) + base + column) = pack8(h[i], tag);
+      if (a.scales == nullptr) *reinterpret_cast<uint4*>(static_cast<T*>(a.z_out) + base + column[i]) = pack8(h[i], tag);
     }
     if (a.scales != nullptr) {  // every lane of the warp is here: the run's maximum is a shuffle
       const float s = e4m3_scale(run_max(on[i] ? magnitude8(h[i]) : 0u));
       if (on[i]) {
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.z_out) + base + column) = quantize8(h[i], __fdiv_rn(1.0f, s));
-        if ((t & 15) == 0) a.scales[row * a.scales_row + (column >> 7) * a.scales_group] = s;
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.z_out) + base + column[i]) = quantize8(h[i], __fdiv_rn(1.0f, s));
+        if ((threadIdx.x & 15) == 0) a.scales[row * a.scales_row + (column[i] >> 7) * a.scales_group] = s;
       }
     }
   }
 }
 
-template <typename T, int TPR, int VPT>
+template <typename T, int VPT, int kMaxThreads, int kMinBlocks>
 int launch_shape(const NormArgs& a, cudaStream_t stream) {
-  constexpr int kThreads = TPR < 128 ? 128 : TPR;
-  constexpr int kRowsPerBlock = kThreads / TPR;
-  const int64_t blocks = (a.rows + kRowsPerBlock - 1) / kRowsPerBlock;
-  if (a.branch != nullptr) sq_block_norm_kernel<T, TPR, VPT, true><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(a);
-  else sq_block_norm_kernel<T, TPR, VPT, false><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(a);
+  const int threads = (a.width / 8 + VPT * 32 - 1) / (VPT * 32) * 32;
+  const unsigned blocks = static_cast<unsigned>(a.rows);
+  if (a.branch != nullptr) sq_block_norm_kernel<T, VPT, true, kMaxThreads, kMinBlocks><<<blocks, threads, 0, stream>>>(a);
+  else sq_block_norm_kernel<T, VPT, false, kMaxThreads, kMinBlocks><<<blocks, threads, 0, stream>>>(a);
   const cudaError_t err = cudaGetLastError();
   return err == cudaSuccess ? SQ_OK : static_cast<int>(err);
 }
 
-// Threads per row and vectors per thread: a warp per row while a lane then holds at most four vectors, else the fewest
-// threads that hold the row in four vectors each.
+// One vector per thread up to 1024 elements, else two; registers are held to what lets 64 / 48 warps live on an SM (the more
+// rows under way, the better HBM is used, until values spill).  Measured at 32768 x 4096 fp16 with fp32 modulation: two vectors
+// and 32 / 40 / 48 / 64 warps 259 / 233 / 236 / 289 us, one vector and 64 warps 247; at 4096 x 5120 with a modulation row per
+// token 72 / 72 / 61 / 62 us; at 32 x 1024 one vector 2.4 us, two 3.2.
 template <typename T>
 int launch_typed(const NormArgs& a, cudaStream_t stream) {
-  const int vectors = a.width / 8;
-  if (vectors <= 32) return launch_shape<T, 32, 1>(a, stream);
-  if (vectors <= 64) return launch_shape<T, 32, 2>(a, stream);
-  if (vectors <= 128) return launch_shape<T, 32, 4>(a, stream);
-  if (vectors <= 256) return launch_shape<T, 128, 2>(a, stream);
-  if (vectors <= 384) return launch_shape<T, 128, 3>(a, stream);
-  if (vectors <= 512) return launch_shape<T, 128, 4>(a, stream);
-  if (vectors <= 768) return launch_shape<T, 256, 3>(a, stream);
-  if (vectors <= 1024) return launch_shape<T, 256, 4>(a, stream);
-  if (vectors <= 1536) return launch_shape<T, 512, 3>(a, stream);
-  return launch_shape<T, 512, 4>(a, stream);
+  if (a.width <= 512) return launch_shape<T, 1, 64, 32>(a, stream);
+  if (a.width <= 1024) return launch_shape<T, 1, 128, 16>(a, stream);
+  if (a.width <= 2048) return launch_shape<T, 2, 128, 12>(a, stream);
+  if (a.width <= 4096) return launch_shape<T, 2, 256, 6>(a, stream);
+  if (a.width <= 8192) return launch_shape<T, 2, 512, 3>(a, stream);
+  return launch_shape<T, 2, 1024, 1>(a, stream);
 }
 
 // ---------------------------------------------------------------------------------------------- e4m3 quantizer
