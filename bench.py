@@ -157,6 +157,71 @@ def measure_int8_peak(device):
 DIT_WORKLOADS = {"dit_a8": (8, False), "dit_a4": (4, True)}
 
 
+def run_dit_fp8(args):
+    """The stack with e4m3 linears, AdaLN modulation with gates and rotary positions: one denoising step captured and
+    replayed as one CUDA graph, ms per step (lower is better), with the whole clip copied in and the result out beside it."""
+    if args.impl == "reference":
+        print(json.dumps({"impl": "reference", "unavailable": "the reference has no fp8 linear, no rotary positions and no model"}), flush=True)
+        return
+    if not torch.cuda.is_available():
+        raise SystemExit("bench.py needs a CUDA device: the B200 path has no CPU fallback.")
+    if args.gpus != 1:
+        raise SystemExit("dit_fp8 runs on one GPU.")
+    import __graft_entry__ as entry
+    entry.load_package()
+    from fastwamjoint_quantization_b200 import dit, native
+    device = torch.device("cuda", 0)
+    cfg = dit.DiTConfig(linear="fp8", modulated=True, rotary=True)
+    model = dit.SyntheticDiT(cfg, device=device, backend="native")
+    x = torch.randn(1, cfg.tokens, cfg.hidden, generator=torch.Generator(device=device).manual_seed(0), device=device).bfloat16()
+    x_host = x.cpu().pin_memory()
+    out_host = torch.empty_like(x_host).pin_memory()
+    with torch.no_grad():
+        parity = dit.extended_parity(model, x)
+        for _ in range(max(args.warmup, 3)):
+            model(x)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured = model(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        sampler = ClockSampler(0)
+        sampler.start()
+        events = [torch.cuda.Event(enable_timing=True) for _ in range(4)]
+        events[0].record()
+        for _ in range(args.steps):
+            graph.replay()
+        events[1].record()
+        torch.cuda.synchronize()
+        ms = events[0].elapsed_time(events[1]) / args.steps
+        e2e_steps = max(3, min(args.steps, 20))
+        events[2].record()
+        for _ in range(e2e_steps):
+            x.copy_(x_host, non_blocking=True)
+            graph.replay()
+            out_host.copy_(captured, non_blocking=True)
+        events[3].record()
+        torch.cuda.synchronize()
+        e2e_ms = events[2].elapsed_time(events[3]) / e2e_steps
+    clocks = sampler.stop()
+    status = native.device_status()
+    if status != 0:
+        raise SystemExit(f"a kernel gave up a bounded wait: device status {status}")
+    linear_ops = 2.0 * cfg.tokens * cfg.blocks * cfg.hidden * (4 * cfg.hidden + 2 * cfg.ffn)
+    print(json.dumps({
+        "metric": "30-block e4m3 DiT step ms (graph)", "value": ms, "unit": "ms", "n_gpus": 1, "steps": args.steps,
+        "warmup": max(args.warmup, 3), "ms_per_step": ms, "higher_is_better": False, "scaling": "weak", "vs_baseline": None,
+        "dtype": "e4m3 linears, bf16 attention", "data": "synthetic",
+        "config": {"workload": "dit_fp8", "blocks": cfg.blocks, "hidden": cfg.hidden, "heads": cfg.heads, "ffn": cfg.ffn,
+                   "tokens": cfg.tokens, "launch": "one CUDA graph per step", "l2": "3.4 GB of weights streamed per step (> 126 MB L2)"},
+        # per block: two norms, a product of their codes each, two linears (quantizer and product), rotary; the last norm
+        "gpu_launches": (9 * cfg.blocks + 1) * args.steps,
+        "linear_tflops": linear_ops / (ms * 1e-3) / 1e12,
+        "e2e": {"value": e2e_ms, "unit": "ms", "h2d_bytes_per_step": x_host.numel() * 2, "d2h_bytes_per_step": out_host.numel() * 2},
+        "clocks": clocks, "parity": parity}), flush=True)
+
+
 def measured_peaks():
     """(HBM GB/s, source) from MEASURED_PEAKS.json, else the documented fallback."""
     peaks_file = ROOT / "MEASURED_PEAKS.json"
@@ -526,7 +591,7 @@ def main():
     parser.add_argument("--gpus", type=int, default=1)
     parser.add_argument("--steps", type=int, default=200)
     parser.add_argument("--warmup", type=int, default=10)
-    parser.add_argument("--workload", default="c2", choices=sorted(WORKLOADS) + sorted(DIT_WORKLOADS) +
+    parser.add_argument("--workload", default="c2", choices=sorted(WORKLOADS) + sorted(DIT_WORKLOADS) + ["dit_fp8"] +
                         ["nsplit_ffn_up", "c5_sweep", "m4096_ffn_up_channel"])
     parser.add_argument("--impl", default="b200", choices=["b200", "reference"])
     parser.add_argument("--no-cpu-baseline", action="store_true")
@@ -547,6 +612,11 @@ def main():
         if args.steps == 200:
             args.steps = 20
         (run_sweep if args.workload == "c5_sweep" else run_channel)(args)
+        return
+    if args.workload == "dit_fp8":
+        if args.steps == 200:
+            args.steps = 20
+        run_dit_fp8(args)
         return
     if args.workload in DIT_WORKLOADS:
         if args.steps == 200:

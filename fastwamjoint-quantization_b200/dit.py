@@ -2,11 +2,14 @@
 3072->9216, attention out 3072->3072, FFN 3072->12288 (GELU) ->3072, RMSNorm, residuals; batch 1 with 1560
 latent + 32 action tokens.  Every linear is a ``TokenQuantLinear`` (int4 weights with fp16 group-128 scales,
 per-token int8 or int4 activations, optional block-local 128-point rotation); attention stays in bf16
-(``scaled_dot_product_attention``).  The reference's model (FastWAMJoint) is not available, so the weights are
+(``scaled_dot_product_attention``).  ``DiTConfig`` also takes the rest of a video model's block: e4m3 linears with a
+scale for each block of 128 (``linear="fp8"``), AdaLN modulation with a gate behind each branch (``modulated``) and rotary
+positions on time, height and width with the norm of q and k in front (``rotary``).  The reference's model (FastWAMJoint) is not available, so the weights are
 random (N(0, 0.02), per-layer seeds) and the stack exists to measure and check one captured denoising step.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 import torch
@@ -15,8 +18,9 @@ import torch.nn.functional as F
 
 from . import native
 from .kernels.w4a8.ops import pack_signed_int4
-from .quant import GROUP, quantize_weight_group
+from .quant import GROUP, dequantize_weight_block, fake_quant_token_runs, quantize_weight_block, quantize_weight_group
 from .rht import randomized_block_hadamard_transform, rht_signs, rotate_weight_
+from .rotary import even_sections, grid_positions, rotary_frequencies, rotary_reference
 
 
 class TokenQuantLinear(nn.Module):
@@ -127,6 +131,37 @@ class TokenQuantLinear(nn.Module):
         return F.linear(qx, self._reference_weight(x.dtype), self.bias)
 
 
+class BlockScaledLinear(nn.Module):
+    """e4m3 linear: weight scales for blocks of 128 x 128, activation scales for each token and run of 128.
+
+    ``backend="native"`` runs the B200 kernels on a bf16 / fp16 input (quantized on the way) or on the ``(codes, scales)``
+    pair ``native.block_norm(quantize=True)`` gives; ``backend="reference"`` is the fake-quant form in plain torch, which
+    takes values only."""
+
+    def __init__(self, weight: torch.Tensor, *, bias: torch.Tensor | None = None, backend: str = "native"):
+        super().__init__()
+        codes, scales = quantize_weight_block(weight)
+        self.register_buffer("weight", codes)
+        self.register_buffer("weight_scales", scales)
+        self.register_buffer("bias", bias)
+        self.out_features, self.in_features = weight.shape
+        self.dtype, self.backend = weight.dtype, backend
+
+    def forward(self, x, *, input_activation: str | None = None) -> torch.Tensor:
+        if self.backend == "native":
+            if isinstance(x, tuple):
+                return native.fp8_gemm(*x, self.weight, self.weight_scales, self.bias, out_dtype=self.dtype)
+            return native.fp8_linear(x, self.weight, self.weight_scales, self.bias, input_activation=input_activation)
+        values = x.float()
+        if input_activation == "gelu":
+            values = F.gelu(values)
+        rows = fake_quant_token_runs(values.reshape(-1, self.in_features))
+        y = rows @ dequantize_weight_block(self.weight, self.weight_scales).t()
+        if self.bias is not None:
+            y = y + self.bias.float()
+        return y.to(self.dtype).reshape(*x.shape[:-1], self.out_features)
+
+
 @dataclass(frozen=True)
 class DiTConfig:
     blocks: int = 30
@@ -138,6 +173,21 @@ class DiTConfig:
     latent_tokens: int = 1560
     action_tokens: int = 32
     eps: float = 1e-6
+    linear: str = "int4"        # "int4": TokenQuantLinear, "fp8": BlockScaledLinear
+    modulated: bool = False     # AdaLN scale and shift in front of each branch, a gate behind it
+    rotary: bool = False        # positions on (time, height, width), q and k normed per head
+    grid: tuple = (3, 20, 26)   # latent tokens along each axis (rotary)
+
+    def __post_init__(self):
+        if self.linear not in ("int4", "fp8"):
+            raise ValueError("linear must be 'int4' or 'fp8'.")
+        if self.rotary and math.prod(self.grid) != self.latent_tokens:
+            raise ValueError("the grid must cover the latent tokens.")
+
+    @property
+    def plain(self) -> bool:
+        """The benchmark configurations' block: int4 linears, no modulation, no positions."""
+        return self.linear == "int4" and not self.modulated and not self.rotary
 
     @property
     def tokens(self) -> int:
@@ -162,12 +212,62 @@ class DiTBlock(nn.Module):
         for j, op in enumerate(self.OPERATIONS):
             generator = torch.Generator(device=device).manual_seed(1000 + 4 * index + j)
             weight = (torch.randn(shapes[op], generator=generator, device=device) * 0.02).to(dtype)
-            layers[op] = TokenQuantLinear(weight, activation_bits=config.activation_bits, rotate=config.rotate,
-                                          module_name=f"blocks.{index}.{op}", backend=backend)
+            if config.linear == "fp8":
+                layers[op] = BlockScaledLinear(weight, backend=backend)
+            else:
+                layers[op] = TokenQuantLinear(weight, activation_bits=config.activation_bits, rotate=config.rotate,
+                                              module_name=f"blocks.{index}.{op}", backend=backend)
         self.qkv, self.o, self.up, self.down = (layers[op] for op in self.OPERATIONS)
+        self.backend = backend
+        modulation = None
+        if config.modulated:  # rows: shift, scale, gate of the attention branch, then of the FFN's
+            generator = torch.Generator(device=device).manual_seed(500 + index)
+            modulation = (torch.randn(1, 6, h, generator=generator, device=device) * 0.1).to(dtype)
+            modulation[:, [2, 5]] += 1.0  # gates around one: the branches carry
+        self.register_buffer("modulation", modulation)
+
+    def _norms(self, x, branch, gate, scale, shift, last: bool = False):
+        """``(stream, input of the next linear)``: the branch before joins the stream under its gate, the norm of the
+        result is modulated and - e4m3 linears - quantized."""
+        cfg = self.config
+        quantize = cfg.linear == "fp8" and self.backend == "native" and not last
+        if self.backend == "native":
+            return native.block_norm(x, branch, gate=gate, norm="rms", mod_scale=scale, mod_shift=shift, eps=cfg.eps,
+                                     quantize=quantize)
+        h = x.float()
+        if branch is not None:
+            h = h + (branch.float() if gate is None else gate.float() * branch.float())
+        z = h * torch.rsqrt(h.square().mean(dim=-1, keepdim=True) + cfg.eps)
+        if scale is not None:
+            z = z * (1 + scale.float()) + shift.float()
+        # a quantized input is quantized from the unrounded norm
+        return h.to(x.dtype), z if cfg.linear == "fp8" and not last else z.to(x.dtype)
+
+    def _turned(self, q, k, places):
+        if places is None:
+            return q, k
+        positions, inv_freq, sections = places
+        if self.backend == "native":
+            return native.rotary(q, k, positions, inv_freq, sections=sections, norm="head", eps=self.config.eps)
+        return tuple(rotary_reference(t, positions, inv_freq, sections=sections, norm="head", eps=self.config.eps) for t in (q, k))
+
+    def step(self, x: torch.Tensor, branch=None, gate=None, places=None):
+        """One block of the extended configuration: takes the stream and the last block's FFN branch with its gate,
+        returns the same after this block (``SyntheticDiT.forward`` joins the last one)."""
+        cfg = self.config
+        b, m, h = x.shape
+        shift1, scale1, gate1, shift2, scale2, gate2 = (None,) * 6 if self.modulation is None else self.modulation.unbind(1)
+        x, z = self._norms(x, branch, gate, scale1, shift1)
+        qkv = self.qkv(z).reshape(b, m, 3, cfg.heads, h // cfg.heads)
+        q, k = self._turned(qkv[:, :, 0], qkv[:, :, 1], places)
+        attn = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), qkv[:, :, 2].transpose(1, 2))
+        x, z = self._norms(x, self.o(attn.transpose(1, 2).reshape(b, m, h)), gate1, scale2, shift2)
+        return x, self.down(self.up(z), input_activation="gelu"), gate2
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         cfg = self.config
+        if not cfg.plain:
+            raise RuntimeError("a block with fp8 linears, modulation or positions runs through step().")
         b, m, h = x.shape
         # RMSNorm and GELU ride in the pre-pass of the linear that consumes them (a whole-GPU streaming kernel
         # with ALU to spare); the two residual adds stay elementwise kernels.
@@ -193,6 +293,15 @@ class SyntheticDiT(nn.Module):
             for module in self.modules():
                 if isinstance(module, TokenQuantLinear):
                     module.workspace = self.workspace
+        positions = inv_freq = None
+        if config.rotary:  # latent tokens in raster order; action tokens behind them in time
+            self.sections = even_sections(config.hidden // config.heads)
+            actions = torch.zeros(config.action_tokens, 3, dtype=torch.int32)
+            actions[:, 0] = torch.arange(config.action_tokens) + config.grid[0]
+            positions = torch.cat((grid_positions(*config.grid), actions)).to(device)
+            inv_freq = rotary_frequencies(self.sections, device=device)
+        self.register_buffer("positions", positions, persistent=False)
+        self.register_buffer("inv_freq", inv_freq, persistent=False)
 
     def prepack(self) -> "SyntheticDiT":
         """Give every linear a kernel-native copy of its weight (see ``TokenQuantLinear.prepack``)."""
@@ -203,11 +312,17 @@ class SyntheticDiT(nn.Module):
 
     def set_backend(self, backend: str) -> None:
         for module in self.modules():
-            if isinstance(module, TokenQuantLinear):
+            if isinstance(module, (TokenQuantLinear, BlockScaledLinear, DiTBlock)):
                 module.backend = backend
 
     def forward(self, tokens: torch.Tensor) -> torch.Tensor:
         x = tokens
+        if not self.config.plain:
+            branch = gate = None
+            places = None if self.positions is None else (self.positions, self.inv_freq, self.sections)
+            for block in self.blocks:
+                x, branch, gate = block.step(x, branch, gate, places)
+            return self.blocks[-1]._norms(x, branch, gate, None, None, last=True)[1]
         for block in self.blocks:
             x = block(x)
         return rms_norm(x, self.config.eps)
@@ -241,7 +356,11 @@ def stack_parity(model: SyntheticDiT, tokens: torch.Tensor) -> dict:
                         how one block of the (random, untrained) stack amplifies a flipped activation code.
     ``free_running``    both stacks run from ``tokens`` on their own: error of the native activations after each block.
     ``output``          the summary, errors after the final norm included.  The reference backend's dequantized
-                        weights are freed block by block, so the extra memory is one block's worth."""
+                        weights are freed block by block, so the extra memory is one block's worth.
+
+    For the benchmark configurations' plain blocks; ``extended_parity`` is the counterpart for the others."""
+    if not model.config.plain:
+        raise ValueError("stack_parity compares plain blocks; use extended_parity.")
     report = {"linear": [], "code_mismatch": [], "teacher_forced": [], "free_running": []}
     reference_x = native_x = tokens
     for block in model.blocks:
@@ -278,3 +397,35 @@ def stack_parity(model: SyntheticDiT, tokens: torch.Tensor) -> dict:
                         "teacher_forced_max": max(report["teacher_forced"]),
                         "free_running": _rel_fro(rms_norm(native_x, eps), rms_norm(reference_x, eps))}
     return report
+
+
+@torch.no_grad()
+def extended_parity(model: SyntheticDiT, tokens: torch.Tensor) -> dict:
+    """How far the native blocks of an extended configuration are from its plain-torch backend: relative Frobenius error
+    of each block's stream and branch when both backends get the reference's input of that block (largest over the
+    blocks), and of the output when both run from ``tokens`` on their own."""
+    places = None if model.positions is None else (model.positions, model.inv_freq, model.sections)
+    worst = {"stream": 0.0, "branch": 0.0}
+    x, branch, gate = tokens, None, None
+    for block in model.blocks:
+        modules = [m for m in block.modules() if hasattr(m, "backend")]
+        outs = {}
+        for backend in ("native", "reference"):
+            for m in modules:
+                m.backend = backend
+            outs[backend] = block.step(x, branch, gate, places)
+            for m in modules:  # the int4 linears keep a dequantized copy
+                if isinstance(m, TokenQuantLinear):
+                    m._dequantized = None
+        for m in modules:
+            m.backend = "native"
+        for i, name in enumerate(worst):
+            worst[name] = max(worst[name], _rel_fro(outs["native"][i], outs["reference"][i]))
+        x, branch, gate = outs["reference"]
+    model.set_backend("native")
+    free = model(tokens)
+    reference = model.blocks[-1]
+    reference.backend = "reference"
+    want = reference._norms(x, branch, gate, None, None, last=True)[1]
+    reference.backend = "native"
+    return {"block_stream_max": worst["stream"], "block_branch_max": worst["branch"], "free_running": _rel_fro(free, want)}

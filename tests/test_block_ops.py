@@ -575,6 +575,40 @@ def test_block_operators_in_a_row(native, quant, rope):
     assert rel(h, want_h) < 4 * half_step(torch.bfloat16) and rel(z, want_z) < 4 * half_step(torch.bfloat16)
 
 
+@pytest.fixture(scope="module")
+def dit(pkg):
+    return importlib.import_module(P + "dit")
+
+
+def small_dit(dit, **kw):
+    return dit.DiTConfig(**{**dict(blocks=2, hidden=512, heads=4, ffn=1024, latent_tokens=168, action_tokens=32, grid=(3, 7, 8),
+                                   linear="fp8", modulated=True, rotary=True), **kw})
+
+
+@gpu
+@pytest.mark.parametrize("kw", [{}, {"linear": "int4"}, {"modulated": False}, {"rotary": False}, {"heads": 8, "latent_tokens": 7, "grid": (1, 1, 7)}])
+def test_extended_dit_blocks_against_plain_torch(native, dit, kw):
+    """The stack's blocks with e4m3 linears, modulation and positions, on both backends, and as one graph."""
+    cfg = small_dit(dit, **kw)
+    model = dit.SyntheticDiT(cfg, device="cuda", backend="native")
+    x = randn(1, cfg.tokens, cfg.hidden, dtype=torch.bfloat16)
+    with torch.no_grad():
+        parity = dit.extended_parity(model, x)
+        # On the reference's own input of a block both backends round the same four or five bf16 tensors and the same codes; a
+        # value that lands on the other side of a rounding moves by one step, and what codes flip by it is averaged over K.
+        # The bar of a linear on its own is 1e-2 (test_gpu_modules); a branch chains four of them.
+        assert parity["block_stream_max"] < 1e-2 and parity["block_branch_max"] < 4e-2, parity
+        eager = model(x)
+        graph = torch.cuda.CUDAGraph()
+        static = torch.zeros_like(x)
+        model(static)
+        with torch.cuda.graph(graph):
+            out = model(static)
+        static.copy_(x)
+        graph.replay()
+        assert torch.equal(out, eager)
+
+
 # ---------------------------------------------------------------------------------------------------- refusals
 def test_c_abi_refuses_before_any_launch(pkg):
     """Host-side checks of the C entry points: no GPU needed, the pointers are never read."""
@@ -666,6 +700,26 @@ def test_host_helpers(quant, rope):
     got = rope.rotary_reference(x, positions, f, sections=(1, 2))
     want, _ = plain_rotary(x, positions, f, (1, 2), "interleaved", None, None)
     assert (got.double() - want).abs().max() <= 16 * U * x.abs().max()
+
+
+def test_extended_dit_on_the_cpu(dit):
+    """The plain-torch backend needs no GPU; what a configuration refuses."""
+    cfg = small_dit(dit, hidden=64, heads=2, ffn=128, latent_tokens=12, action_tokens=4, grid=(2, 2, 3))
+    model = dit.SyntheticDiT(cfg, device="cpu", backend="reference")
+    x = torch.randn(1, 16, 64, generator=torch.Generator().manual_seed(0)).bfloat16()
+    y = model(x)
+    assert y.shape == x.shape and y.isfinite().all()
+    assert (y.float().square().mean(-1) - 1).abs().max() < 0.02  # the final norm, rounded to bf16
+    assert not torch.equal(model(x.flip(1)), y.flip(1))  # the positions count
+    with pytest.raises(ValueError, match="grid"):
+        small_dit(dit, grid=(3, 7, 7))
+    with pytest.raises(ValueError, match="linear"):
+        small_dit(dit, linear="int3")
+    with pytest.raises(RuntimeError, match="step"):
+        model.blocks[0](x)
+    with pytest.raises(ValueError, match="extended_parity"):
+        dit.stack_parity(model, x)
+    assert dit.DiTConfig().plain
 
 
 def test_operators_need_the_gpu(native):
