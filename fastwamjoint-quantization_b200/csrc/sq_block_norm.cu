@@ -101,7 +101,7 @@ __device__ __forceinline__ void standardise(float (&v)[VPT][8], const bool (&on)
     squares = row_sum(local_squares(v));
     eps = 0.0f;
   }
-  const float r = rsqrtf(fmaf(squares, inv_width, eps));
+  const float r = __frsqrt_rn(fmaf(squares, inv_width, eps));
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
 #pragma unroll

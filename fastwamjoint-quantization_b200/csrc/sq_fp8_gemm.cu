@@ -39,6 +39,7 @@ struct Fp8Args {
   int64_t M;
   int N, runs;
   int ch_tiles, tok_tiles;
+  int bias_vectors;            // the bias is 16-byte aligned
 };
 
 // ---------------------------------------------------------------------------------------------- PTX of this kernel
@@ -105,12 +106,16 @@ __device__ __forceinline__ void report_timeout(int* status, volatile int* abort_
   if (status != nullptr) atomicCAS(status, 0, code);
 }
 
+// 8 biases, the same in every lane; one load where the caller's bias is on the vector grid
 template <typename T>
-__device__ __forceinline__ void load_bias8(const void* bias, int n, float (&b)[8]) {
-  // element by element: the caller's bias may start anywhere
-  const T* p = static_cast<const T*>(bias) + n;
+__device__ __forceinline__ void load_bias8(const Fp8Args& p, int n, float (&b)[8]) {
+  const T* at = static_cast<const T*>(p.bias) + n;
+  if (p.bias_vectors) {
+    unpack8(__ldg(reinterpret_cast<const uint4*>(at)), b, static_cast<const T*>(nullptr));
+  } else {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) b[e] = static_cast<float>(__ldg(p + e));
+    for (int e = 0; e < 8; ++e) b[e] = static_cast<float>(__ldg(at + e));
+  }
 }
 
 // ---------------------------------------------------------------------------------------------- few tokens
@@ -338,7 +343,7 @@ __global__ void __launch_bounds__(128 + 32 * few_drain_warps(TOK), 1)
     }
     if (p.bias != nullptr) {
       float b[8];
-      load_bias8<OutT>(p.bias, n, b);
+      load_bias8<OutT>(p, n, b);
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] += b[e];
     }
@@ -713,7 +718,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           for (int e = 0; e < 8; ++e) y[e] = sums[part * 32 + c * 8 + e];
           if (p.bias != nullptr && n + c * 8 < p.N) {
             float b[8];
-            load_bias8<OutT>(p.bias, n + c * 8, b);
+            load_bias8<OutT>(p, n + c * 8, b);
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] += b[e];
           }
@@ -978,6 +983,7 @@ int launch_fp8_gemm(const Fp8GemmArgs& a, cudaStream_t stream) {
   p.scales_group = a.scales_group;
   p.weight_scales = a.weight_scales;
   p.bias = a.bias;
+  p.bias_vectors = aligned16_host(a.bias);
   p.out = a.out;
   p.status = device_status_word();
   if (p.status == nullptr) return SQ_ERR_DRIVER;

@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(256) sq_rotary_kernel(const RotaryArgs a) {
       for (int h = threadIdx.x & 31; h < count_heads; h += 32) s += sums[(i >> 1) * all_heads + begin + h];
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-      if ((threadIdx.x & 31) == 0) roots[i] = rsqrtf(s / (static_cast<float>(count_heads) * static_cast<float>(a.dim)) + a.eps);
+      if ((threadIdx.x & 31) == 0) roots[i] = __frsqrt_rn(s / (static_cast<float>(count_heads) * static_cast<float>(a.dim)) + a.eps);
     }
   };
   const bool once = items <= kAtOnce * segments;  // the block's items fit its threads' registers: no second reading
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(256) sq_rotary_kernel(const RotaryArgs a) {
       if (kHead) {
         float s = squares(u[n], v[n]);
         for (int d = lanes >> 1; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        scale = rsqrtf(fmaf(s, a.inv_dim, a.eps));
+        scale = __frsqrt_rn(fmaf(s, a.inv_dim, a.eps));
       }
       if (item >= items || !on) continue;
       const Item it = decode(item);
