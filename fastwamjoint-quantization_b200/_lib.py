@@ -6,6 +6,8 @@ present when a kernel is requested, the call raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import struct
 from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 from functools import lru_cache
@@ -133,6 +135,22 @@ def load_library() -> ctypes.CDLL:
         fn.restype = restype
         fn.argtypes = argtypes
     return lib
+
+
+@lru_cache(maxsize=1)
+def load_binding():
+    """``sq_binding.so`` (``csrc/sq_binding.cpp``), the short way into the library for ordinary calls of the block operators,
+    or None where it has not been built: the ctypes way serves every call."""
+    path = LIB_PATH.with_name("sq_binding.so")
+    if not path.exists():
+        return None
+    load_library()
+    import torch  # noqa: F401  (the module links its libraries)
+    loader = importlib.machinery.ExtensionFileLoader("sq_binding", str(path))
+    spec = importlib.util.spec_from_file_location("sq_binding", str(path), loader=loader)
+    module = importlib.util.module_from_spec(spec)
+    loader.exec_module(module)
+    return module
 
 
 def status_string(status: int) -> str:

@@ -5,20 +5,28 @@
 The library has a C ABI only (``include/sq_b200.h``); it links the CUDA runtime
 statically and needs neither PyTorch nor libcuda at link time (the one driver
 call it makes, ``cuTensorMapEncodeTiled``, is looked up at run time).
+
+Beside it goes ``sq_binding.so``, a small CPython module over that C ABI which takes the
+block operators' ordinary calls (``csrc/sq_binding.cpp``); it is compiled by the host
+compiler against PyTorch's headers.
 """
 from __future__ import annotations
 
 import argparse
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 LIB = HERE / "lib" / "libsq_b200.so"
+BINDING = HERE / "lib" / "sq_binding.so"
+BINDING_SOURCE = CSRC / "sq_binding.cpp"
 SOURCES = ("sq_prepass.cu", "sq_gemm_tc.cu", "sq_gemm_ts.cu", "sq_fp8_gemm.cu", "sq_block_norm.cu", "sq_rotary.cu",
            "sq_api.cu")
 HEADERS = ("sq_internal.h", "sq_ptx.cuh", "sq_rows.cuh", "../../include/sq_b200.h")
@@ -41,8 +49,34 @@ def stale() -> bool:
     return any(d.stat().st_mtime > built for d in deps)
 
 
+def build_binding(force: bool = False, verbose: bool = False) -> Path:
+    """``sq_binding.so``, linked against the built library (found beside it at run time) and PyTorch's own."""
+    deps = [BINDING_SOURCE, (CSRC / "../../include/sq_b200.h").resolve(), Path(__file__)]
+    if not force and BINDING.exists() and all(d.stat().st_mtime <= BINDING.stat().st_mtime for d in deps):
+        return BINDING
+    spec = importlib.util.find_spec("torch")
+    compiler = shutil.which("g++")
+    if spec is None or compiler is None:
+        raise RuntimeError("PyTorch and g++ are needed to build sq_binding.so.")
+    torch_dir = Path(spec.origin).parent
+    cuda = Path(nvcc()).resolve().parents[1]
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [compiler, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-isystem", str(torch_dir / "include"),
+           "-isystem", str(torch_dir / "include/torch/csrc/api/include"), "-isystem", str(cuda / "include"),
+           "-I", sysconfig.get_paths()["include"], str(BINDING_SOURCE), "-o", str(tmp), f"-L{LIB.parent}", f"-l:{LIB.name}",
+           f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN"]
+    done = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or done.returncode:
+        sys.stderr.write(done.stdout + done.stderr)
+    if done.returncode:
+        raise RuntimeError("building sq_binding.so failed")
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     if not force and not stale():
+        build_binding(verbose=verbose)
         return LIB
     obj_dir = HERE / "build"
     obj_dir.mkdir(exist_ok=True)
@@ -72,6 +106,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         sys.stderr.write(done.stdout + done.stderr)
         raise RuntimeError("linking libsq_b200.so failed")
     os.replace(tmp, LIB)
+    build_binding(force=force, verbose=verbose)
     return LIB
 
 

@@ -251,8 +251,10 @@ def linear(x: torch.Tensor, packed: torch.Tensor, w_scales: torch.Tensor, bias, 
 
 
 # ---------------------------------------------------------------------------------------- operators of a block
-# The smallest calls of these operators take 3 us on the device, so what the host does per call is their cost: properties
-# are read once, arguments go to C as one structure filled by position, the stream is asked for by device index.
+# The smallest calls of these operators take 2 to 5 us on the device, so what the host does per call is their cost.  Each
+# wrapper offers its call to the binding first (``csrc/sq_binding.cpp``), which launches it if it is an ordinary one and answers
+# None if not; the Python below takes those - views to copy, outputs given, refusals - and everything where the binding is not
+# built.  There properties are read once, arguments go to C packed by position, the stream is asked for by device index.
 RUN = 128  # k that share a scale in the e4m3 product, and the rows of a weight block
 _E4M3 = torch.float8_e4m3fn
 
@@ -264,6 +266,22 @@ def _no_gradient(*tensors) -> None:
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError("the B200 operators have no backward pass: call them under torch.no_grad() or detach the inputs.")
+
+
+class _Binding:
+    """The binding's functions, looked up at the first call; ``enabled = False`` sends every call the Python way."""
+    enabled = True
+    _module = False
+
+    def __call__(self, name: str, *args):
+        if self._module is False:
+            self._module = _lib.load_binding()
+        if self._module is None or not self.enabled:
+            return None
+        return getattr(self._module, name)(*args)
+
+
+_binding = _Binding()
 
 
 def _call(name: str, device: torch.device, *args) -> None:
@@ -290,6 +308,10 @@ def _require_rows(x: torch.Tensor, name: str = "x") -> None:
         _require_cuda(x, name)
     if x.dtype not in _DTYPES or x.ndim < 2:
         raise ValueError(f"{name} must be a bf16 or fp16 tensor with token and channel axes.")
+
+
+def _round256(n: int) -> int:
+    return (n + 255) & ~255
 
 
 _ACTIVATIONS = {None: _lib.ACT_FN_NONE, "gelu": _lib.ACT_FN_GELU}
@@ -352,6 +374,8 @@ def fp8_gemm(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, we
     """e4m3 codes [..., K] (with fp32 ``scales`` [rows, ceil(K / 128)], any strides) x e4m3 weight [N, K] (with fp32
     ``weight_scales`` [ceil(N / 128), ceil(K / 128)], one per 128 x 128 block) + bias -> [..., N] in ``out_dtype``.  Sums in
     fp32, one rounding.  ``quant.quantize_weight_block`` makes the weight's form, ``fp8_quantize`` the codes'."""
+    if out is None and (y := _binding("fp8_gemm", codes, scales, weight, weight_scales, bias, out_dtype)) is not None:
+        return y
     if not codes.is_cuda:
         _require_cuda(codes, "codes")
     _no_gradient(scales, weight_scales, bias, out)
@@ -382,6 +406,8 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tenso
     """``linear([gelu](x))`` in e4m3: ``fp8_quantize`` and ``fp8_gemm`` as one call, the product's set-up and first weight
     loads running under the quantizer.  ``workspace`` (uint8, at least ``sq_fp8_workspace_bytes(rows, K)``) may be passed
     to reuse a buffer across calls that are ordered on the device; the weight must be ready before the call."""
+    if out is None and workspace is None and (y := _binding("fp8_linear", x, weight, weight_scales, bias, input_activation)) is not None:
+        return y
     _require_rows(x)
     _no_gradient(x, weight_scales, bias, out)
     activation = _input_activation(input_activation)
@@ -390,7 +416,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tenso
     n = _check_fp8_weight(device, k, weight, weight_scales, bias, dtype)
     x = _vectors(x)
     rows = x.numel() // k
-    nbytes = _lib.load_library().sq_fp8_workspace_bytes(rows, k)
+    nbytes = _round256(rows * k) + _round256(rows * -(-k // RUN) * 4)  # sq_fp8_workspace_bytes
     if workspace is None:
         workspace = x.new_empty((nbytes,), dtype=torch.uint8)
     elif (workspace.dtype != torch.uint8 or workspace.device != device or workspace.numel() < nbytes
@@ -466,6 +492,9 @@ def block_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *, gate=None
     [width]; gate, mod_scale and mod_shift [..., width], each row for an equal share of x's rows (a strided slice of a
     modulation table is read in place), all in x's dtype or fp32.  ``quantize`` gives z as ``(codes, scales)`` for
     ``fp8_gemm`` (``fp8_quantize``'s rule, no rounding to x's dtype between).  ``out`` takes h; it may be x or branch."""
+    if out is None and (pair := _binding("block_norm", x, branch, gate, residual_scale, post_norm, post_weight, post_bias, norm,
+                                         weight, bias, mod_scale, mod_shift, eps, quantize)) is not None:
+        return pair
     _require_rows(x)
     _no_gradient(x, branch, gate, post_weight, post_bias, weight, bias, mod_scale, mod_shift, out)
     if norm not in _NORMS or post_norm not in _NORMS:
@@ -570,6 +599,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     heads of a token ("token", weights [heads * dim]), statistics in fp32 (values up to 2^59).  ``out`` is a pair (q, k) of
     tensors to write, strided as a cache or a transposed view may be; they may be the inputs themselves, but overlap
     nothing otherwise."""
+    if out is None and (pair := _binding("rotary", q, k, positions, inv_freq, sections, layout, norm, q_weight, k_weight, eps)) is not None:
+        return pair
     if not q.is_cuda:
         _require_cuda(q, "q")
     if q.ndim != 4 or q.dtype not in _DTYPES:

@@ -125,6 +125,24 @@ def test_fp8_gemm_writes_its_rows_and_nothing_else(native, quant):
 
 
 @gpu
+@pytest.mark.parametrize("m", [5, 300, 1100])
+def test_fp8_bias_off_the_vector_grid_and_strided_codes(native, quant, m):
+    n, k = 264, 512
+    _, codes, scales, weight, weight_scales, bias = fp8_case(quant, m, n, k, torch.bfloat16)
+    want = native.fp8_gemm(codes, scales, weight, weight_scales, bias, out_dtype=torch.bfloat16)
+    shifted = torch.zeros(n + 1, device="cuda", dtype=torch.bfloat16)
+    shifted[1:] = bias
+    wide = torch.zeros(m, 2 * k, device="cuda", dtype=torch.uint8)
+    wide[:, :k] = codes.view(torch.uint8)
+    got = native.fp8_gemm(wide.view(torch.float8_e4m3fn)[:, :k], scales.contiguous(), weight, weight_scales, shifted[1:],
+                          out_dtype=torch.bfloat16)
+    assert torch.equal(got, want)
+    one = scales[:, :1].expand(m, scales.shape[1])  # one scale per token, broadcast over the runs
+    got = native.fp8_gemm(codes, one, weight, weight_scales, out_dtype=torch.bfloat16)
+    assert torch.equal(got, native.fp8_gemm(codes, one.contiguous(), weight, weight_scales, out_dtype=torch.bfloat16))
+
+
+@gpu
 def test_fp8_non_finite_values_stay_in_their_rows(native, quant):
     m, n, k = 40, 256, 384
     x, _, _, weight, weight_scales, _ = fp8_case(quant, m, n, k, torch.bfloat16)
@@ -607,6 +625,108 @@ def test_extended_dit_blocks_against_plain_torch(native, dit, kw):
         static.copy_(x)
         graph.replay()
         assert torch.equal(out, eager)
+
+
+CAPTURE_FIRST = '''
+import importlib, sys
+import torch
+sys.path.insert(0, {root!r})
+import __graft_entry__ as entry
+entry.load_package()
+native = importlib.import_module("fastwamjoint_quantization_b200.native")
+x = torch.randn(64, 512, device="cuda").bfloat16()
+w = torch.randn(256, 512, device="cuda").to(torch.float8_e4m3fn)
+ws = torch.ones(2, 4, device="cuda")
+q = torch.randn(1, 64, 4, 128, device="cuda").bfloat16()
+pos = torch.arange(64, device="cuda", dtype=torch.int32)[:, None]
+f = torch.ones(64, device="cuda", dtype=torch.float64)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = native.fp8_linear(x, w, ws)
+    big = native.fp8_linear(x.repeat(32, 1), w, ws)
+    h, z = native.block_norm(x, x)
+    r, _ = native.rotary(q, None, pos, f, sections=(64,))
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(y, native.fp8_linear(x, w, ws)) and torch.equal(big[:64], big[64:128])
+assert torch.equal(z, native.block_norm(x, x)[1]) and torch.equal(r, native.rotary(q, None, pos, f, sections=(64,))[0])
+assert native.device_status() == 0
+print("captured first")
+'''
+
+
+@gpu
+def test_first_call_of_a_process_under_capture():
+    """Nothing a first call does (attributes, occupancy, symbol and driver lookups) is refused while a stream is captured."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    root = str(Path(__file__).resolve().parents[1])
+    done = subprocess.run([sys.executable, "-c", CAPTURE_FIRST.format(root=root)], capture_output=True, text=True, timeout=180)
+    assert done.returncode == 0 and "captured first" in done.stdout, done.stderr[-2000:]
+
+
+@gpu
+def test_binding_and_python_way_give_the_same(native, quant, rope):
+    """The ordinary calls that the binding takes, against the Python way on the same inputs; that it takes them, and leaves
+    what is not ordinary."""
+    module = native._lib.load_binding()
+    assert module is not None, "sq_binding.so is not built"
+    x, codes, scales, weight, weight_scales, bias = fp8_case(quant, 48, 264, 512, torch.bfloat16)
+    branch = randn(48, 512, seed=9, dtype=torch.bfloat16)
+    table = randn(4, 3, 512, seed=10, dtype=torch.bfloat16)
+    w32 = randn(512, seed=11)
+    qkv = randn(2, 24, 12, 64, seed=12, dtype=torch.bfloat16)
+    positions = rope.grid_positions(2, 3, 4, device="cuda")
+    freq = rope.rotary_frequencies((12, 10, 10), device="cuda")
+    calls = [
+        lambda: native.fp8_gemm(codes, scales, weight, weight_scales, bias, out_dtype=torch.bfloat16),
+        lambda: native.fp8_gemm(codes.view(2, 24, 512), scales.contiguous(), weight, weight_scales, out_dtype=torch.float16),
+        lambda: native.fp8_linear(x, weight, weight_scales, bias, input_activation="gelu"),
+        lambda: native.block_norm(x.view(4, 12, 512), norm="layer", mod_scale=table[:, 1], mod_shift=table[:, 0], quantize=True),
+        lambda: native.block_norm(x, branch, gate=w32, norm=None, post_norm="rms", post_weight=w32, post_bias=table[0, 0]),
+        lambda: native.block_norm(x, branch, gate=table[:, 2:3], residual_scale=0.5, weight=w32, bias=w32, eps=1e-3),
+        lambda: native.rotary(qkv[:, :, :6], qkv[:, :, 6:8], positions, freq, sections=(12, 10, 10), layout="half", norm="head", q_weight=w32[:64]),
+        lambda: native.rotary(qkv, None, positions.long()[None], freq, sections=(12, 10, 10)),
+    ]
+    flat = lambda t: [] if t is None else [t] if isinstance(t, torch.Tensor) else [u for v in t for u in flat(v)]
+    for call in calls:
+        fast = flat(call())
+        native._binding.enabled = False
+        try:
+            slow = flat(call())
+        finally:
+            native._binding.enabled = True
+        assert len(fast) == len(slow)
+        for a, b in zip(fast, slow):
+            assert a.shape == b.shape and a.dtype == b.dtype and a.stride() == b.stride()
+            assert torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+    assert module.fp8_linear(x, weight, weight_scales, bias, None) is not None
+    for odd in (x.t().contiguous().t(), x.cpu(), x.float(), x[:0], x.clone().requires_grad_(), x[:, :508], "x"):
+        assert module.fp8_linear(odd, weight, weight_scales, bias, None) is None
+    assert module.fp8_linear(x, weight, weight_scales) is None  # another number of arguments
+    assert module.fp8_linear(x, weight, weight_scales, bias, "relu") is None
+    assert module.rotary(qkv, None, positions, freq, [12, 10, 10], "interleaved", None, None, None, 1e-6) is None  # sections: a tuple
+    assert module.rotary(qkv, None, positions, freq, (33,), "interleaved", None, None, None, 1e-6) is None
+    assert native.rotary(qkv, None, positions, freq, sections=[12, 10, 10])[1] is None
+
+
+@gpu
+def test_two_streams_at_once(native, quant):
+    """Calls on two streams, unordered: each has its own outputs and workspaces."""
+    x, _, _, weight, weight_scales, bias = fp8_case(quant, 512, 1024, 1024, torch.bfloat16)
+    want = native.fp8_linear(x, weight, weight_scales, bias)
+    want_h, want_z = native.block_norm(x, x)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for i in range(20):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append((native.fp8_linear(x, weight, weight_scales, bias), *native.block_norm(x, x)))
+    torch.cuda.synchronize()
+    for y, h, z in got:
+        assert torch.equal(y, want) and torch.equal(h, want_h) and torch.equal(z, want_z)
 
 
 # ---------------------------------------------------------------------------------------------------- refusals
