@@ -11,9 +11,10 @@
 //
 // A block takes some tokens; a head is covered by `lanes` lanes (a power of two), each with a chunk of it: 8 neighbouring
 // elements (4 pairs), or - pairs half a head apart - 8 or 4 neighbours and their partners, so that no lane needs another's
-// elements (pairs no multiple of 4: 8 of them, element by element).  The kernel is near its issue slots besides HBM: the weights
-// of the head norm are multiplied into the token's table of turns (once per token instead of once per head), and a lane's loads of several heads are issued before the first is used.  The norm over a token's
-// heads reads the token twice, the second time out of the L1.
+// elements (pairs no multiple of 4: 8 of them, element by element).  The kernel is near its issue slots besides HBM: the
+// weights of the head norm are multiplied into the token's table of turns (once per token instead of once per head), and a
+// lane's loads of several heads are issued before the first is used.  The norm over a token's heads reads a token that does
+// not fit its block's registers twice, the second time out of the L1.
 #include "sq_internal.h"
 #include "sq_rows.cuh"
 
@@ -394,7 +395,8 @@ int launch_mode(RotaryArgs a, int64_t batch, cudaStream_t stream) {
   // takes as many as its threads hold at one time
   const int64_t tokens = a.length * batch;
   int per_block = 512 / a.dim > 0 ? 512 / a.dim : 1;
-  while (per_block > 1 && tokens / per_block < 4 * 148) --per_block;
+  constexpr int kFewBlocks = 4 * 148;  // four for each SM
+  while (per_block > 1 && tokens / per_block < kFewBlocks) --per_block;
   if (kNorm == SQ_ROTARY_NORM_TOKEN)
     while (per_block > 1 && per_block * all_heads > 4 * (256 >> a.lanes_log2)) --per_block;
   a.tokens_per_block = per_block;
@@ -448,6 +450,9 @@ int launch_rotary(const SqRotary& r, cudaStream_t stream) {
     a.section_end[x] = end;
   }
   if (end < 1 || 2 * end > r.dim) return SQ_ERR_SHAPE;
+  int64_t lanes = 1;
+  while (8 * lanes < r.dim) lanes *= 2;
+  if ((static_cast<int64_t>(r.heads) + r.kv_heads) * lanes > 4096) return SQ_ERR_SHAPE;  // items of a block stay below 2^20
   for (const void* p : {r.q, r.k, static_cast<const void*>(r.q_out), static_cast<const void*>(r.k_out), r.q_weight, r.k_weight})
     if (!aligned16_host(p)) return SQ_ERR_SHAPE;
   for (const int64_t* s : {r.q_strides, r.k_strides, r.q_out_strides, r.k_out_strides})

@@ -49,44 +49,6 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8], const __half*) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Eight fp32 values as four packed pairs: one instruction per pair for a sum, a product or both.
-struct Pairs {
-  uint64_t p[4];
-};
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-  return static_cast<uint64_t>(__float_as_uint(lo)) | (static_cast<uint64_t>(__float_as_uint(hi)) << 32);
-}
-__device__ __forceinline__ float pair_lo(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
-__device__ __forceinline__ float pair_hi(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-template <typename T>
-__device__ __forceinline__ void unpack_pairs(const uint4& raw, Pairs& v, const T* tag) {
-  float f[8];
-  unpack8(raw, f, tag);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v.p[i] = pair(f[2 * i], f[2 * i + 1]);
-}
-template <typename T>
-__device__ __forceinline__ uint4 pack_pairs(const Pairs& v, const T* tag) {
-  const float f[8] = {pair_lo(v.p[0]), pair_hi(v.p[0]), pair_lo(v.p[1]), pair_hi(v.p[1]),
-                      pair_lo(v.p[2]), pair_hi(v.p[2]), pair_lo(v.p[3]), pair_hi(v.p[3])};
-  return pack8(f, tag);
-}
-
 // data read once: past the L1, so that the parameter rows every token rereads stay there
 __device__ __forceinline__ uint4 load_stream(const void* p) {
   uint4 v;
@@ -105,17 +67,6 @@ __device__ __forceinline__ void load_params(const void* base, int64_t index, boo
     v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   } else {
     unpack8(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(base) + index)), v, static_cast<const T*>(nullptr));
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void load_param_pairs(const void* base, int64_t index, bool f32, Pairs& v) {
-  if (f32) {
-    const ulonglong2* p = reinterpret_cast<const ulonglong2*>(static_cast<const float*>(base) + index);
-    const ulonglong2 a = __ldg(p), b = __ldg(p + 1);
-    v.p[0] = a.x; v.p[1] = a.y; v.p[2] = b.x; v.p[3] = b.y;
-  } else {
-    unpack_pairs(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(base) + index)), v, static_cast<const T*>(nullptr));
   }
 }
 

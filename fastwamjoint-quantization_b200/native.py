@@ -405,7 +405,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tenso
                workspace: torch.Tensor | None = None) -> torch.Tensor:
     """``linear([gelu](x))`` in e4m3: ``fp8_quantize`` and ``fp8_gemm`` as one call, the product's set-up and first weight
     loads running under the quantizer.  ``workspace`` (uint8, at least ``sq_fp8_workspace_bytes(rows, K)``) may be passed
-    to reuse a buffer across calls that are ordered on the device; the weight must be ready before the call."""
+    to reuse a buffer across calls that are ordered on the device."""
     if out is None and workspace is None and (y := _binding("fp8_linear", x, weight, weight_scales, bias, input_activation)) is not None:
         return y
     _require_rows(x)
@@ -429,6 +429,19 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tenso
         _call("sq_fp8_linear", device, x.data_ptr(), _DTYPES[dtype], rows, k, n, activation, weight.data_ptr(),
               weight_scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), workspace.data_ptr(), nbytes)
     return out
+
+
+def _refuse_overlap(out: torch.Tensor, same, others) -> None:
+    """``out`` is written while other rows are still read: it may be one of ``same`` itself, but share no memory with them or
+    with ``others`` otherwise."""
+    begin = out.data_ptr()
+    end = begin + out.numel() * out.element_size()
+    for t in (*(t for t in same if t.data_ptr() != begin), *others):
+        if t is None or t.numel() == 0:
+            continue
+        at = t.data_ptr()
+        if at < end and begin < at + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size():
+            raise ValueError("out must be x or branch itself, or share no memory with the inputs.")
 
 
 _ABSENT = (0, 0, 0, 0, 0)
@@ -491,7 +504,8 @@ def block_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *, gate=None
     Norms are "rms" or "layer", their statistics in fp32 from the unrounded h, both with ``eps``.  Weights and biases are
     [width]; gate, mod_scale and mod_shift [..., width], each row for an equal share of x's rows (a strided slice of a
     modulation table is read in place), all in x's dtype or fp32.  ``quantize`` gives z as ``(codes, scales)`` for
-    ``fp8_gemm`` (``fp8_quantize``'s rule, no rounding to x's dtype between).  ``out`` takes h; it may be x or branch."""
+    ``fp8_gemm`` (``fp8_quantize``'s rule, no rounding to x's dtype between).  ``out`` takes h; it may be x or branch itself,
+    and shares no memory with an input otherwise."""
     if out is None and (pair := _binding("block_norm", x, branch, gate, residual_scale, post_norm, post_weight, post_bias, norm,
                                          weight, bias, mod_scale, mod_shift, eps, quantize)) is not None:
         return pair
@@ -512,6 +526,7 @@ def block_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *, gate=None
     x_rows = _vectors(x)
     rows = x.numel() // width
     kept = []  # copies made for alignment live until the launch
+    parameters = (gate, post_weight, post_bias, weight, bias, mod_scale, mod_shift)
     gate, mod_scale, mod_shift = (_row_param(t, kept, rows, width, dtype, device, name) for t, name in (
         (gate, "gate"), (mod_scale, "mod_scale"), (mod_shift, "mod_shift")))
     post_weight, post_bias, weight, bias = (_channel_param(t, kept, width, dtype, device, name) for t, name in (
@@ -522,7 +537,11 @@ def block_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *, gate=None
         if branch.shape != shape or branch.dtype is not dtype or branch.device != device:
             raise ValueError("branch must match x's shape, dtype and device.")
         branch = _vectors(branch)
-        h = torch.empty_like(x_rows) if out is None else _checked_output(out, shape, dtype, device)
+        if out is None:
+            h = torch.empty_like(x_rows)
+        else:
+            h = _checked_output(out, shape, dtype, device)
+            _refuse_overlap(h, (x_rows, branch), parameters)
         branch_ptr, h_ptr = branch.data_ptr(), h.data_ptr()
     if norm is not None:
         z = torch.empty_like(x_rows, dtype=_E4M3) if quantize else torch.empty_like(x_rows)

@@ -668,6 +668,19 @@ def test_first_call_of_a_process_under_capture():
 
 
 @gpu
+def test_out_may_be_an_input_but_not_part_of_one(native):
+    buffer = randn(9, 64, seed=3, dtype=torch.bfloat16)
+    x, branch = buffer[:8], randn(8, 64, seed=4, dtype=torch.bfloat16)
+    want, _ = native.block_norm(x, branch)
+    for bad in (dict(out=buffer[1:]), dict(out=branch, gate=branch), dict(out=x, mod_scale=x[:1]), dict(out=x, weight=x[7])):
+        with pytest.raises(ValueError, match="share no memory"):
+            native.block_norm(x, branch, **bad)
+    kept = buffer.clone()
+    h, _ = native.block_norm(x, branch, out=branch)
+    assert h is branch and torch.equal(h, want) and torch.equal(buffer, kept)
+
+
+@gpu
 def test_binding_and_python_way_give_the_same(native, quant, rope):
     """The ordinary calls that the binding takes, against the Python way on the same inputs; that it takes them, and leaves
     what is not ordinary."""
@@ -785,6 +798,8 @@ def test_c_abi_refuses_before_any_launch(pkg):
         assert rotary(**kw) == lib_mod.ERR_NULL
     for kw in ({"dtype": 2}, {"layout": 2}, {"norm": 3}, {"position_type": 3}, {"q_weight": ok}):
         assert rotary(**kw) == lib_mod.ERR_ENUM
+    for kw in ({"heads": 1023, "kv_heads": 2}, {"heads": 1 << 30}, {"heads": 2049, "kv_heads": 0, "dim": 16, "sections": (8,), "axes": 1}):
+        assert rotary(**kw) == lib_mod.ERR_SHAPE
     odd = (lib_mod.c_int64 * 3)(512, 64, 36)
     for kw in ({"dim": 36}, {"dim": 264}, {"heads": 0}, {"axes": 0}, {"axes": 5}, {"q": off}, {"k_out": off}, {"q_strides": odd},
                {"k_out_strides": odd}, {"positions": 4097}, {"inv_freq": 4100}, {"sections": (8, 9)}, {"sections": (0, 0)},
