@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(256) sq_rotary_kernel(const RotaryArgs a) {
       if (kHead) {
         float s = squares(u[n], v[n]);
         for (int d = lanes >> 1; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        scale = __frsqrt_rn(fmaf(s, a.inv_dim, a.eps));
+        scale = rsqrtf(fmaf(s, a.inv_dim, a.eps));  // once per head and lane: the correctly rounded root costs 11 us of 162
       }
       if (item >= items || !on) continue;
       const Item it = decode(item);
