@@ -237,14 +237,15 @@ int launch_typed(const NormArgs& a, cudaStream_t stream) {
 }
 
 // ---------------------------------------------------------------------------------------------- e4m3 quantizer
-// 16 lanes per run of 128, kRuns runs per thread loaded before the first is used (64 bytes in flight per thread).  No row
-// statistics are needed, so runs are dealt out regardless of rows; the row of a run is a multiplication by the
-// reciprocal of the runs per row (exact for run numbers below 2^31).
-constexpr int kRuns = 4;
+// 16 lanes per run of 128, kRuns runs per thread loaded before the first is used.  No row statistics are needed, so runs are
+// dealt out regardless of rows; the row of a run is a multiplication by the reciprocal of the runs per row (exact for run
+// numbers below 2^31).  Two runs and registers for eight blocks per SM: four runs at five blocks take 2.3 us instead of 1.8
+// for one token of 4096, 62.9 instead of 64.4 for 8192 of 14336, and with the activation 114 instead of 109.
+constexpr int kRuns = 2;
 constexpr int kQuantThreads = 256;
 
 template <typename T, bool kGelu>
-__global__ void __launch_bounds__(kQuantThreads) sq_fp8_quantize_kernel(
+__global__ void __launch_bounds__(kQuantThreads, 8) sq_fp8_quantize_kernel(
     const T* __restrict__ x, uint8_t* __restrict__ codes, float* __restrict__ scales, int64_t scales_row,
     int64_t scales_group, uint32_t runs, uint32_t runs_per_row, uint32_t magic, uint32_t shift, int width) {
   // the product behind this kernel may set itself up meanwhile; it waits for this grid before it reads anything of it
@@ -267,10 +268,7 @@ __global__ void __launch_bounds__(kQuantThreads) sq_fp8_quantize_kernel(
   for (int i = 0; i < kRuns; ++i) {
     float v[8];
     unpack8(raw[i], v, static_cast<const T*>(nullptr));
-    if (kGelu) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = gelu_erf(v[e]);
-    }
+    if (kGelu) gelu8(v);
     const float s = e4m3_scale(run_max(magnitude8(v)));
     if (on[i]) {
       const int64_t at = static_cast<int64_t>(row[i]) * width + static_cast<int64_t>(group[i]) * 128 + lane16 * 8;

@@ -1,5 +1,5 @@
 // Row helpers shared by the block-norm, e4m3 quantizer and rotary kernels: 8-element vectors of bf16 / fp16 / fp32, e4m3
-// conversion with the scale of a run of 128, erf GELU.
+// conversion with the scale of a run of 128, GELU.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -106,7 +106,54 @@ __device__ __forceinline__ uint32_t run_max(uint32_t m) {
   return m;
 }
 
-__device__ __forceinline__ float gelu_erf(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f)); }
+// Two fp32 values in one register pair: one instruction for both products or sums.
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  return static_cast<uint64_t>(__float_as_uint(lo)) | (static_cast<uint64_t>(__float_as_uint(hi)) << 32);
+}
+__device__ __forceinline__ float low2(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float high2(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, float c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(pack2(c, c)));
+  return d;
+}
+
+// erf GELU, x * Phi(x), of 8 values.  With a = |x| and t = 1 / (1 + 0.306 a):
+//   x * Phi(x) = (x < 0 ? 0 : x) - a * Phi(-a),   a * Phi(-a) = a * t * exp(-a^2 / 2) * P(t)
+// Phi(-a) exp(a^2 / 2) is smooth in t over all of 0 .. 1, so one polynomial serves every x; P was fitted to the function in
+// 64 bits for the least relative error (1.1e-7).  In fp32 the whole is within 5e-7 of its value down to x = -3 and 2e-6
+// to -8: unlike x / 2 * (1 + erf(x / sqrt 2)) nothing cancels where x is negative.  The quantizer is bound by its issue
+// slots with the activation (20.0 us for 1592 x 12288, 11.6 without): with erff it took 28.7, with this one value at a time
+// 22.0, with one reciprocal for four values 21.3.
+__device__ __forceinline__ void gelu8(float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const uint64_t a = pack2(fminf(fabsf(v[i]), 64.0f), fminf(fabsf(v[i + 1]), 64.0f));  // 64: infinity times zero stays out
+    const uint64_t d = fma2(a, pack2(0.306f, 0.306f), 1.0f);
+    const uint64_t power = mul2(mul2(a, a), pack2(-0.72134752044448170f, -0.72134752044448170f));  // -log2(e) / 2
+    float t0, t1, e0, e1;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t0) : "f"(low2(d)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t1) : "f"(high2(d)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(low2(power)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(high2(power)));
+    const uint64_t t = pack2(t0, t1);
+    uint64_t p = fma2(t, pack2(0.036538217f, 0.036538217f), -0.15070112f);
+    p = fma2(p, t, 0.17938644f);
+    p = fma2(p, t, -0.033036616f);
+    p = fma2(p, t, 0.11862919f);
+    p = fma2(p, t, 0.10436764f);
+    p = fma2(p, t, 0.122772194f);
+    p = fma2(p, t, 0.1220441f);
+    const uint64_t h = mul2(mul2(mul2(a, t), pack2(e0, e1)), p);
+    v[i] = fmaf(v[i], v[i] < 0.0f ? 0.0f : 1.0f, -low2(h));  // x * 0, not 0: -infinity gives NaN as the formula does
+    v[i + 1] = fmaf(v[i + 1], v[i + 1] < 0.0f ? 0.0f : 1.0f, -high2(h));
+  }
+}
 
 inline bool aligned16_host(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

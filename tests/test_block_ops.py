@@ -6,6 +6,7 @@ every output is rounded once.  To it comes the error of fp32 arithmetic, counted
 that were added: stated where each bound is written."""
 import importlib
 import itertools
+import math
 
 import pytest
 import torch
@@ -188,6 +189,30 @@ def test_fp8_linear_is_quantizer_and_product(native, quant, m, n, k, gelu):
         s = scales.double().repeat_interleave(128, dim=1)[:, :k]
         err = (codes.double() * s - value).abs()
         assert (err <= value.abs() * 2.0 ** -4 * (1 + 1e-5) + s * 2.0 ** -10 + 16 * U * x.double().abs()).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gelu_of_every_value(native, dtype):
+    """Every finite 16-bit value, one per run so that its code is 448 and its scale carries the activation: what the kernel
+    computes of x * Phi(x) to fp32.  The bound: fit 1.1e-7; t 2 U (reciprocal and sum), exp 2 U and its argument 2 U of
+    x^2 / 2, eight products and sums of P at U each, four products, the scale's two divisions."""
+    bits = torch.arange(-32768, 32768, dtype=torch.int32, device="cuda").to(torch.int16).view(dtype)
+    x = bits[torch.isfinite(bits)]
+    x = x[: x.numel() // 16 * 16].contiguous()
+    rows = torch.zeros(x.numel(), 128, device="cuda", dtype=dtype)
+    rows[:, 0] = x
+    codes, scales = native.fp8_quantize(rows, input_activation="gelu")
+    exact = x.double() * torch.special.ndtr(x.double())
+    seen = exact.abs() > 448e-8  # below, the scale is the floor's
+    got = codes[:, 0].double().sign() * scales[:, 0].double() * 448
+    assert (codes[seen, 0].float().abs() == 448).all() and not codes[:, 1:].float().any()
+    bound = 1.1e-7 + U * (20 + x.double() ** 2 * (x < 0))
+    assert ((got - exact).abs()[seen] <= (bound * exact.abs())[seen]).all()
+    odd = torch.zeros(4, 128, device="cuda", dtype=dtype)
+    odd[0, 5], odd[1, 5], odd[2, 5] = math.inf, -math.inf, math.nan
+    scales = native.fp8_quantize(odd, input_activation="gelu")[1].cpu()[:, 0]
+    assert torch.isinf(scales[0]) and torch.isnan(scales[1:3]).all() and scales[3] == 1e-8
 
 
 @gpu
