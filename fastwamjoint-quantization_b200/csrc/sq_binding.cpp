@@ -160,7 +160,7 @@ SqParam rows_param(const Device& d, PyObject* o, const Tensor& x, int64_t rows) 
     groups = t.numel() / width;
   }
   need(groups > 0 && rows % groups == 0 && stride >= 0 && stride % 8 == 0);
-  q.data = d.take(t, 16);
+  q.data = d.take(t, f32 ? 32 : 16);
   q.row_stride = stride;
   q.span = rows / groups;
   q.is_fp32 = f32;
@@ -172,7 +172,7 @@ SqParam channel_param(const Device& d, PyObject* o, const Tensor& x) {
   const Tensor& t = tensor_of(o);
   const bool f32 = t.scalar_type() == at::kFloat;
   need((f32 || t.scalar_type() == x.scalar_type()) && t.dim() == 1 && t.size(0) == x.size(-1) && t.is_contiguous());
-  q.data = d.take(t, 16);
+  q.data = d.take(t, f32 ? 32 : 16);
   q.is_fp32 = f32;
   return q;
 }
@@ -246,7 +246,7 @@ const void* rotary_weight(const Device& d, PyObject* o, const Tensor& q, int64_t
   *f32 = t.scalar_type() == at::kFloat;
   need(norm != SQ_ROTARY_NORM_NONE && (*f32 || t.scalar_type() == q.scalar_type()) && t.dim() == 1 && t.is_contiguous() &&
        t.size(0) == (norm == SQ_ROTARY_NORM_TOKEN ? count * q.size(3) : q.size(3)));
-  return d.take(t, 16);
+  return d.take(t, *f32 ? 32 : 16);
 }
 
 // (q, k, positions, inv_freq, sections, layout, norm, q_weight, k_weight, eps)

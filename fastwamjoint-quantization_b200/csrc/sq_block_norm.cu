@@ -224,7 +224,7 @@ int launch_shape(const NormArgs& a, cudaStream_t stream) {
 
 // One vector per thread up to 1024 elements, else two; registers are held to what lets 64 / 48 warps live on an SM (the more
 // rows under way, the better HBM is used, until values spill).  Measured at 32768 x 4096 fp16 with fp32 modulation: two vectors
-// and 32 / 40 / 48 / 64 warps 259 / 233 / 236 / 289 us, one vector and 64 warps 247; at 4096 x 5120 with a modulation row per
+// and 32 / 40 / 48 / 64 warps 259 / 233 / 236 / 289 us, one vector and 64 warps 247 (48 warps with 32-byte parameter loads: 227); at 4096 x 5120 with a modulation row per
 // token 72 / 72 / 61 / 62 us; at 32 x 1024 one vector 2.4 us, two 3.2.
 template <typename T>
 int launch_typed(const NormArgs& a, cudaStream_t stream) {
@@ -343,7 +343,7 @@ int launch_block_norm(const SqBlockNorm& b, cudaStream_t stream) {
   a.mod_scale = take(b.mod_scale);
   a.mod_shift = take(b.mod_shift);
   for (const Param& q : {a.gate, a.post_weight, a.post_bias, a.weight, a.bias, a.mod_scale, a.mod_shift})
-    if (!aligned16_host(q.p)) return SQ_ERR_SHAPE;  // vectors of 8 elements
+    if (!aligned_param_host(q.p, q.f32 != 0)) return SQ_ERR_SHAPE;
   if (b.rows == 0) return SQ_OK;
   a.x = b.x;
   a.branch = b.branch;

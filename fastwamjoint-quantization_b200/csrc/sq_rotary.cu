@@ -453,8 +453,9 @@ int launch_rotary(const SqRotary& r, cudaStream_t stream) {
   int64_t lanes = 1;
   while (8 * lanes < r.dim) lanes *= 2;
   if ((static_cast<int64_t>(r.heads) + r.kv_heads) * lanes > 4096) return SQ_ERR_SHAPE;  // items of a block stay below 2^20
-  for (const void* p : {r.q, r.k, static_cast<const void*>(r.q_out), static_cast<const void*>(r.k_out), r.q_weight, r.k_weight})
+  for (const void* p : {r.q, r.k, static_cast<const void*>(r.q_out), static_cast<const void*>(r.k_out)})
     if (!aligned16_host(p)) return SQ_ERR_SHAPE;
+  if (!aligned_param_host(r.q_weight, r.q_weight_fp32 != 0) || !aligned_param_host(r.k_weight, r.k_weight_fp32 != 0)) return SQ_ERR_SHAPE;
   for (const int64_t* s : {r.q_strides, r.k_strides, r.q_out_strides, r.k_out_strides})
     for (int i = 0; i < 3; ++i) {
       if ((s == r.k_strides || s == r.k_out_strides) && r.kv_heads == 0) continue;

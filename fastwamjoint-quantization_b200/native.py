@@ -457,8 +457,8 @@ def _channel_param(t, kept: list, width: int, dtype, device, name: str):
     if t.shape != (width,):
         raise ValueError(f"{name} must be [{width}].")
     pointer = t.data_ptr()
-    if pointer % 16 or not t.is_contiguous():
-        t = _vectors(t)
+    if pointer % (32 if f32 else 16) or not t.is_contiguous():  # 8 parameters are one load
+        t = t.clone(memory_format=torch.contiguous_format)
         kept.append(t)
         pointer = t.data_ptr()
     return (pointer, 0, 0, f32, 0)
@@ -481,8 +481,8 @@ def _row_param(t, kept: list, rows: int, width: int, dtype, device, name: str):
         raise ValueError(f"{name} rows must cover complete input rows: {groups} rows for {rows}.")
     stride, step = t.stride()
     pointer = t.data_ptr()
-    if step != 1 or stride % 8 or pointer % 16:
-        t = _vectors(t)
+    if step != 1 or stride % 8 or pointer % (32 if f32 else 16):
+        t = t.clone(memory_format=torch.contiguous_format)
         kept.append(t)
         pointer, stride = t.data_ptr(), width
     return (pointer, stride, rows // groups if rows else 1, f32, 0)
@@ -597,8 +597,8 @@ def _rotary_weight(t, kept: list, count: int, dim: int, norm, dtype, device, nam
     if t.device != device or not (f32 or t.dtype is dtype) or t.shape != ((count * dim,) if norm == "token" else (dim,)):
         raise ValueError(f"{name} must be [dim] (head norm) or [heads * dim] (token norm), in q's dtype or float32, on its device.")
     pointer = t.data_ptr()
-    if pointer % 16 or not t.is_contiguous():
-        t = _vectors(t)
+    if pointer % (32 if f32 else 16) or not t.is_contiguous():  # 8 parameters are one load
+        t = t.clone(memory_format=torch.contiguous_format)
         kept.append(t)
         pointer = t.data_ptr()
     return pointer, f32

@@ -312,7 +312,7 @@ int sq_fp8_linear(const void* x, int x_dtype, int64_t rows, int64_t K, int64_t N
                   void* stream);
 size_t sq_fp8_workspace_bytes(int64_t rows, int64_t K);
 
-/* Rows of parameters: [width] elements in the rows' type (is_fp32 = 0) or fp32, 16-byte aligned; data null: absent. */
+/* Rows of parameters: [width] elements in the rows' type (is_fp32 = 0) or fp32, 16-byte aligned (fp32: 32); data null: absent. */
 typedef struct SqParam {
   const void* data;
   int64_t row_stride; /* elements between rows (a multiple of 8); ignored for per-channel vectors */

@@ -706,6 +706,26 @@ def test_out_may_be_an_input_but_not_part_of_one(native):
 
 
 @gpu
+@pytest.mark.parametrize("offset", [1, 4, 8])
+def test_parameters_of_any_alignment(native, offset):
+    """Parameters whose address is off the kernels' vectors of 16 or 32 bytes give what aligned ones do."""
+    x, branch = (randn(6, 136, seed=i, dtype=torch.bfloat16) for i in (1, 2))
+    def off(t):
+        flat = torch.zeros(t.numel() + offset, device="cuda", dtype=t.dtype)
+        flat[offset:] = t.flatten()
+        return flat[offset:].view(t.shape)
+    for dtype in (torch.float32, torch.bfloat16):
+        table, w = randn(3, 136, seed=3, dtype=dtype), randn(136, seed=4, dtype=dtype)
+        want = native.block_norm(x, branch, gate=table, post_norm="rms", post_weight=w, weight=w, mod_shift=table)
+        got = native.block_norm(x, branch, gate=off(table), post_norm="rms", post_weight=off(w), weight=off(w), mod_shift=off(table))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        q, w = randn(1, 6, 2, 64, seed=5, dtype=torch.bfloat16), randn(128, seed=6, dtype=dtype)
+        turn = lambda w: native.rotary(q, None, torch.arange(6, device="cuda", dtype=torch.int32)[:, None], torch.ones(32, device="cuda", dtype=torch.float64),
+                                       sections=(32,), norm="token", q_weight=w)[0]
+        assert torch.equal(turn(off(w)), turn(w))
+
+
+@gpu
 def test_binding_and_python_way_give_the_same(native, quant, rope):
     """The ordinary calls that the binding takes, against the Python way on the same inputs; that it takes them, and leaves
     what is not ordinary."""
@@ -805,7 +825,7 @@ def test_c_abi_refuses_before_any_launch(pkg):
         assert norm(**kw) == lib_mod.ERR_ENUM
     for kw in ({"x": off}, {"branch": off}, {"h_out": off}, {"z_out": off}, {"width": 60}, {"width": 16392}, {"rows": -1}, {"rows": 1 << 31},
                {"width": 72, "scales": ok}, {"scales": 4097}, {"gate": lib_mod.Param(off, 0, 4)}, {"gate": lib_mod.Param(ok, 0, 0)},
-               {"gate": lib_mod.Param(ok, 4, 1)}, {"weight": lib_mod.Param(off)}):
+               {"gate": lib_mod.Param(ok, 4, 1)}, {"weight": lib_mod.Param(off)}, {"weight": lib_mod.Param(ok + 16, 0, 0, 1)}):
         assert norm(**kw) == lib_mod.ERR_SHAPE
     assert norm(rows=0) == lib_mod.OK
 
