@@ -42,7 +42,9 @@ struct RotaryArgs {
   int lanes_log2, chunks, tokens_per_block;
   int table_rows;           // of a token's table: a lane's pairs, one row each
   int table_lanes;          // entries of a row
-  uint32_t heads_magic;     // item / (heads + kv_heads) = high word of item * this (items below 2^20)
+  // n / d as the high word of n * ceil(2^32 / d), exact while n * d < 2^32 (0: d is 1)
+  uint32_t heads_magic;     // d = heads + kv_heads up to 4096, items below 2^20
+  uint32_t token_magic, row_magic;  // d = a token's table entries, a row's: no more than 512 + 32 entries in all
   float eps, inv_dim;
 };
 
@@ -58,6 +60,8 @@ __device__ __forceinline__ float one_param(const void* base, int64_t index, bool
 __device__ __forceinline__ float one_param(const void* base, int64_t index, bool f32, const __half*) {
   return f32 ? __ldg(static_cast<const float*>(base) + index) : __half2float(__ldg(static_cast<const __half*>(base) + index));
 }
+
+__device__ __forceinline__ int quotient(int n, uint32_t magic) { return magic == 0 ? n : static_cast<int>(__umulhi(n, magic)); }
 
 // C elements of 16 bits, as loaded
 template <int C>
@@ -151,7 +155,8 @@ __global__ void __launch_bounds__(256) sq_rotary_kernel(const RotaryArgs a) {
   const int64_t first_token = static_cast<int64_t>(blockIdx.x - batch * a.blocks_per_batch) * a.tokens_per_block;
   const int here = static_cast<int>(min(static_cast<int64_t>(a.tokens_per_block), a.length - first_token));
   for (int i = threadIdx.x; i < here * half; i += 256) {
-    const int token = i / half, at_row = (i - token * half) / a.table_lanes, j = (i - token * half - at_row * a.table_lanes) * a.table_rows + at_row;
+    const int token = quotient(i, a.token_magic), entry = i - token * half;
+    const int at_row = quotient(entry, a.row_magic), j = (entry - at_row * a.table_lanes) * a.table_rows + at_row;
     float2 cs = make_float2(1.0f, 0.0f);  // interleaved, pairs past `pairs` are not turned
     if (j < a.pairs) {
       int axis = 0;
@@ -197,7 +202,7 @@ __global__ void __launch_bounds__(256) sq_rotary_kernel(const RotaryArgs a) {
   };
   auto decode = [&](int item) {
     Item it;
-    it.token = a.heads_magic == 0 ? item : static_cast<int>(__umulhi(item, a.heads_magic));  // 0: one head, an item is a token
+    it.token = quotient(item, a.heads_magic);
     const int h = item - it.token * all_heads;
     it.is_q = h < a.heads;
     it.head = it.is_q ? h : h - a.heads;
@@ -390,7 +395,10 @@ int launch_mode(RotaryArgs a, int64_t batch, cudaStream_t stream) {
   while ((1 << a.lanes_log2) < a.chunks) ++a.lanes_log2;
   a.table_rows = kHalf ? C : 4;
   a.table_lanes = kHalf ? (a.pairs + C - 1) / C : a.dim / 8;
-  a.heads_magic = all_heads == 1 ? 0 : static_cast<uint32_t>(((uint64_t{1} << 32) + all_heads - 1) / all_heads);
+  auto magic = [](int d) { return d == 1 ? 0u : static_cast<uint32_t>(((uint64_t{1} << 32) + d - 1) / d); };
+  a.heads_magic = magic(all_heads);
+  a.token_magic = magic(a.table_rows * a.table_lanes);
+  a.row_magic = magic(a.table_lanes);
   // tokens of a block: angles for all its threads, but no fewer blocks than a few per SM; the norm over a token's heads
   // takes as many as its threads hold at one time
   const int64_t tokens = a.length * batch;
