@@ -240,7 +240,9 @@ int launch_shape(const NormArgs& a, cudaStream_t stream) {
 // One vector per thread up to 1024 elements, else two; registers are held to what lets 64 / 48 warps live on an SM (the more
 // rows under way, the better HBM is used, until values spill).  Measured at 32768 x 4096 fp16 with fp32 modulation: two vectors
 // and 32 / 40 / 48 / 64 warps 259 / 233 / 236 / 289 us, one vector and 64 warps 247 (48 warps with 32-byte parameter loads: 227); at 4096 x 5120 with a modulation row per
-// token 72 / 72 / 61 / 62 us; at 32 x 1024 one vector 2.4 us, two 3.2.
+// token 72 / 72 / 61 / 62 us; at 32 x 1024 one vector 2.4 us, two 3.2.  Beyond 8192 a block of two vectors per thread fills an
+// SM, and two blocks of four vectors overlap one's loads with the other's sums: 232 us instead of 257 at 8192 x 12288, 259
+// instead of 275 at 8192 x 16384, but 8.2 instead of 5.7 where 64 rows leave SMs idle.
 template <typename T>
 int launch_typed(const NormArgs& a, cudaStream_t stream) {
   if (a.width <= 512) return launch_shape<T, 1, 64, 32>(a, stream);
@@ -248,6 +250,7 @@ int launch_typed(const NormArgs& a, cudaStream_t stream) {
   if (a.width <= 2048) return launch_shape<T, 2, 128, 12>(a, stream);
   if (a.width <= 4096) return launch_shape<T, 2, 256, 6>(a, stream);
   if (a.width <= 8192) return launch_shape<T, 2, 512, 3>(a, stream);
+  if (a.rows >= 2 * 148) return launch_shape<T, 4, 512, 2>(a, stream);
   return launch_shape<T, 2, 1024, 1>(a, stream);
 }
 

@@ -384,6 +384,17 @@ def test_block_norm_groups_of_rows(native, rows, groups):
 
 
 @gpu
+@pytest.mark.parametrize("width", [8208, 12288, 13504, 16384])
+@pytest.mark.parametrize("rows", [295, 296])
+def test_block_norm_wide_rows(native, rows, width):
+    """Rows beyond 8192 elements, with and without a block for each SM's second place."""
+    x, branch = randn(rows, width, dtype=torch.bfloat16), randn(rows, width, seed=1, dtype=torch.bfloat16)
+    table = randn(rows, width, seed=2, scale=0.3)
+    check_block_norm(native, x, branch, post_norm="layer", gate=table[:1], norm="layer", mod_scale=table, mod_shift=table[1:2])
+    check_block_norm(native, x, norm="rms", mod_scale=table, quantize=True)
+
+
+@gpu
 def test_block_norm_hard_rows(native):
     """A large mean, constant rows, zeros, the smallest and the largest values, non-finite values in single rows."""
     x = randn(12, 1024, scale=0.01)
