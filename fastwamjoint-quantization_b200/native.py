@@ -269,16 +269,33 @@ def _no_gradient(*tensors) -> None:
 
 
 class _Binding:
-    """The binding's functions, looked up at the first call; ``enabled = False`` sends every call the Python way."""
-    enabled = True
-    _module = False
+    """The binding's functions as attributes, looked up at the first call of any; ``enabled = False`` sends every call the
+    Python way."""
+    NAMES = ("fp8_gemm", "fp8_linear", "block_norm", "rotary")
 
-    def __call__(self, name: str, *args):
-        if self._module is False:
-            self._module = _lib.load_binding()
-        if self._module is None or not self.enabled:
-            return None
-        return getattr(self._module, name)(*args)
+    def __init__(self):
+        for name in self.NAMES:
+            setattr(self, name, self._first_call(name))
+
+    def _first_call(self, name: str):
+        def call(*args):
+            self.enabled = True
+            return getattr(self, name)(*args)
+        return call
+
+    @property
+    def enabled(self) -> bool:
+        return self.fp8_gemm is not self._decline
+
+    @enabled.setter
+    def enabled(self, on: bool) -> None:
+        module = _lib.load_binding() if on else None
+        for name in self.NAMES:
+            setattr(self, name, self._decline if module is None else getattr(module, name))
+
+    @staticmethod
+    def _decline(*args) -> None:
+        return None
 
 
 _binding = _Binding()
@@ -374,7 +391,7 @@ def fp8_gemm(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, we
     """e4m3 codes [..., K] (with fp32 ``scales`` [rows, ceil(K / 128)], any strides) x e4m3 weight [N, K] (with fp32
     ``weight_scales`` [ceil(N / 128), ceil(K / 128)], one per 128 x 128 block) + bias -> [..., N] in ``out_dtype``.  Sums in
     fp32, one rounding.  ``quant.quantize_weight_block`` makes the weight's form, ``fp8_quantize`` the codes'."""
-    if out is None and (y := _binding("fp8_gemm", codes, scales, weight, weight_scales, bias, out_dtype)) is not None:
+    if out is None and (y := _binding.fp8_gemm(codes, scales, weight, weight_scales, bias, out_dtype)) is not None:
         return y
     if not codes.is_cuda:
         _require_cuda(codes, "codes")
@@ -406,7 +423,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tenso
     """``linear([gelu](x))`` in e4m3: ``fp8_quantize`` and ``fp8_gemm`` as one call, the product's set-up and first weight
     loads running under the quantizer.  ``workspace`` (uint8, at least ``sq_fp8_workspace_bytes(rows, K)``) may be passed
     to reuse a buffer across calls that are ordered on the device."""
-    if out is None and workspace is None and (y := _binding("fp8_linear", x, weight, weight_scales, bias, input_activation)) is not None:
+    if out is None and workspace is None and (y := _binding.fp8_linear(x, weight, weight_scales, bias, input_activation)) is not None:
         return y
     _require_rows(x)
     _no_gradient(x, weight_scales, bias, out)
@@ -506,8 +523,8 @@ def block_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *, gate=None
     modulation table is read in place), all in x's dtype or fp32.  ``quantize`` gives z as ``(codes, scales)`` for
     ``fp8_gemm`` (``fp8_quantize``'s rule, no rounding to x's dtype between).  ``out`` takes h; it may be x or branch itself,
     and shares no memory with an input otherwise."""
-    if out is None and (pair := _binding("block_norm", x, branch, gate, residual_scale, post_norm, post_weight, post_bias, norm,
-                                         weight, bias, mod_scale, mod_shift, eps, quantize)) is not None:
+    if out is None and (pair := _binding.block_norm(x, branch, gate, residual_scale, post_norm, post_weight, post_bias, norm,
+                                                         weight, bias, mod_scale, mod_shift, eps, quantize)) is not None:
         return pair
     _require_rows(x)
     _no_gradient(x, branch, gate, post_weight, post_bias, weight, bias, mod_scale, mod_shift, out)
@@ -618,7 +635,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     heads of a token ("token", weights [heads * dim]), statistics in fp32 (values up to 2^59).  ``out`` is a pair (q, k) of
     tensors to write, strided as a cache or a transposed view may be; they may be the inputs themselves, but overlap
     nothing otherwise."""
-    if out is None and (pair := _binding("rotary", q, k, positions, inv_freq, sections, layout, norm, q_weight, k_weight, eps)) is not None:
+    if out is None and (pair := _binding.rotary(q, k, positions, inv_freq, sections, layout, norm, q_weight, k_weight, eps)) is not None:
         return pair
     if not q.is_cuda:
         _require_cuda(q, "q")
