@@ -782,6 +782,29 @@ def test_binding_and_python_way_give_the_same(native, quant, rope):
 
 
 @gpu
+def test_offsets_past_32_bits(native, quant, rope):
+    """The last rows of tensors of more than 2^31 elements, against the same rows alone."""
+    rows, last = 530000, 200
+    x = torch.empty(rows, 4096, device="cuda", dtype=torch.bfloat16).normal_()
+    end = x[-last:].clone()
+    h, (codes, scales) = native.block_norm(x, x, norm="rms", quantize=True)
+    want_h, (want_codes, want_scales) = native.block_norm(end, end, norm="rms", quantize=True)
+    assert torch.equal(h[-last:], want_h) and torch.equal(scales[-last:], want_scales)
+    assert torch.equal(codes[-last:].view(torch.uint8), want_codes.view(torch.uint8))
+    del h, codes, scales
+    positions = torch.arange(rows, device="cuda")[:, None]
+    turn = lambda t, p: native.rotary(t, None, p, rope.rotary_frequencies((64,), device="cuda"), sections=(64,), norm="head")[0]
+    assert torch.equal(turn(x.view(1, rows, 32, 128), positions)[:, -last:], turn(end.view(1, last, 32, 128), positions[-last:]))
+    weight, weight_scales = quant.quantize_weight_block(randn(4096, 128, scale=0.1))
+    narrow = x[:, :128].contiguous()
+    y = native.fp8_linear(narrow, weight, weight_scales)[-last:].double()
+    want = native.fp8_linear(narrow[-last:].clone(), weight, weight_scales).double()
+    # other tiles, other order of a run's 128 products: 128 U of their magnitudes on either side, and a rounding each
+    size = (narrow[-last:].float().abs() * 1.07) @ quant.dequantize_weight_block(weight, weight_scales).float().abs().t()
+    assert ((y - want).abs() <= 2 * 128 * U * size.double() + 2.0 ** -7 * want.abs()).all()
+
+
+@gpu
 def test_two_streams_at_once(native, quant):
     """Calls on two streams, unordered: each has its own outputs and workspaces."""
     x, _, _, weight, weight_scales, bias = fp8_case(quant, 512, 1024, 1024, torch.bfloat16)
