@@ -578,7 +578,7 @@ const char* sq_status_string(int status) {
     case 9212: return "device: e4m3 product of a pair, MMA warp timed out waiting for a free accumulator";
     case 9213: return "device: e4m3 product of a pair, MMA warp timed out waiting for operands";
     case 9214: return "device: e4m3 product of a pair, drain warp timed out waiting for an accumulator";
-    case 9215: return "device: e4m3 product of a pair, factor warp timed out waiting for a free stage";
+    case 9215: return "device: e4m3 product of a pair, factor warp timed out waiting for a free place";
     case 9216: return "device: e4m3 product of a pair, drain warp timed out waiting for its factors";
     case 9190: return "device: the wait probe gave up, as it is meant to";
     case 9001: return "device: TMA producer timed out waiting for a free stage";

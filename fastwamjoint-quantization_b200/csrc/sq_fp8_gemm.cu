@@ -416,13 +416,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                        const __grid_constant__ CUtensorMap map_out, const Fp8Args p) {
   constexpr int S = pair_stages(BN);
   constexpr int kParts = BN / 128;      // products of 128 channels in a run
-  constexpr int kDepth = 4 / kParts;    // runs whose accumulators fit tensor memory
   constexpr int kCols = BN / 2;         // channels of a drain warp
-  // Batch b of four runs' factors takes the place of batch b - 2: it is written when the MMAs of run 4 b - 5 + kDepth are
-  // done, since these waited for the drain of run 4 b - 5, the last to read that place.  The next phase of the same
-  // barrier, S runs on, waits for the drain of run 4 b - 5 + S >= 4 b and so for this batch: it cannot pass unseen.  (Batch 1
-  // waits for run 2, whose next phase waits for the drain of run 2 + S - kDepth = 5.)
-  static_assert(S >= 5 && kFactorSlots == 8, "two batches of four runs");
+  // Batch b of four runs' factors takes the place of batch b - 2: it is written when the eight drain warps have arrived at
+  // bar_factor_free for that place, each behind its last read of it.  Both barriers of a place are waited for once in each
+  // of their phases by the same warps, so a phase's parity tells it from its neighbours.  (That an MMA of a later run is done
+  // does not free a place: with one product a run the two issuers are not ordered, and the barrier of a run's stage may
+  // still be a round behind, where the same parity has long passed.)
+  static_assert(kFactorSlots == 8, "two batches of four runs");
   constexpr uint32_t kXBytes = kRun * kRun, kWBytes = BN / 2 * kRun;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -432,7 +432,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   const uint32_t bars = factors + kFactorSlots * kFactorBytes;
   const uint32_t bar_full = bars, bar_empty = bars + 8 * S, bar_acc_full = bars + 16 * S, bar_acc_empty = bar_acc_full + 32;
   const uint32_t bar_factor = bar_acc_empty + 32;
-  const uint32_t words = bar_factor + 16;
+  const uint32_t bar_factor_free = bar_factor + 16;
+  const uint32_t words = bar_factor_free + 16;
   volatile uint32_t* tmem_word = reinterpret_cast<volatile uint32_t*>(gen + (words - base));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + (words + 4 - base));
   volatile int* keep_on = reinterpret_cast<volatile int*>(gen + (words + 8 - base));  // an abort flag that nobody sets
@@ -448,7 +449,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       mbar_init(bar_acc_full + 8 * b, 1);
       mbar_init(bar_acc_empty + 8 * b, 16 / kParts);  // the accumulator's drain warps of both thread blocks
     }
-    for (int i = 0; i < 2; ++i) mbar_init(bar_factor + 8 * i, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar_factor + 8 * i, 1);
+      mbar_init(bar_factor_free + 8 * i, 8);  // the drain warps of this thread block
+    }
     *abort_flag = 0;
     *keep_on = 0;
     fence_mbar_init();
@@ -601,8 +605,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
       };
       if (first < tiles) aim();
-      static_assert(3 + kDepth == S, "the first run waited for is the second round of stage 0");
-      uint32_t batch = 0, s = 0, phase = 1;
+      uint32_t batch = 0;
       for (; tile < tiles; ++batch) {
         float t[4][4], w[4][2];
 #pragma unroll
@@ -619,23 +622,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             if (tile < tiles) aim();
           }
         }
-        if (batch == 1) {
-          // nothing is overwritten yet, but a phase is told from its neighbours by parity alone: run 2 done means that the
-          // first round of stage 0 has passed when its second one is waited for next
-          if (!mbar_wait_bounded(bar_empty + 16, 0, abort_flag, kWaitLimitNs)) {
-            if (lane == 0) report_timeout(p.status, abort_flag, 9215);
-            break;
-          }
-        } else if (batch >= 2) {
-          if (!mbar_wait_bounded(bar_empty + 8 * s, phase, abort_flag, kWaitLimitNs)) {
-            if (lane == 0) report_timeout(p.status, abort_flag, 9215);
-            break;
-          }
-          s += 4;
-          if (s >= S) {
-            s -= S;
-            phase ^= 1u;
-          }
+        if (batch >= 2 && !mbar_wait_bounded(bar_factor_free + 8 * (batch & 1u), ((batch >> 1) & 1u) ^ 1u, abort_flag, kWaitLimitNs)) {
+          if (lane == 0) report_timeout(p.status, abort_flag, 9215);
+          break;
         }
         const uint32_t to = factors + (batch & 1u) * 4 * kFactorBytes + lane * 4;
 #pragma unroll
@@ -698,6 +687,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           }
 #pragma unroll
           for (int i = 0; i < 32; ++i) sums[32 * c + i] = fmaf(__uint_as_float(d[c & 1][i]), f, sums[32 * c + i]);
+        }
+        if ((run & 3u) == 3u) {  // this warp has read the batch's factors
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_factor_free + ((run << 1) & 8u));
         }
       }
       int64_t tok;

@@ -1,0 +1,133 @@
+"""The block operators where they can go wrong: the order in which the e4m3 product's warps hand memory to one another, calls
+at the border of what the entry points take, and what they refuse.  Formulas, tolerances and helpers are test_block_ops'."""
+import importlib
+import random
+
+import pytest
+import torch
+
+from test_block_ops import DTYPES, P, fp8_case, fp8_product, fp8_slack, gpu, half_step, no_device_timeouts, randn, within  # noqa: F401
+
+
+@pytest.fixture(scope="module")
+def native(pkg):
+    return importlib.import_module(P + "native")
+
+
+@pytest.fixture(scope="module")
+def quant(pkg):
+    return importlib.import_module(P + "quant")
+
+
+# ------------------------------------------------------------------------- warps of the e4m3 product for many tokens
+class Barrier:
+    """An mbarrier: a phase ends when `count` arrivals are in; a wait names the parity of the phase it waits for."""
+
+    def __init__(self, count):
+        self.count, self.left, self.phase = count, count, 0
+
+    def arrive(self):
+        self.left -= 1
+        if self.left == 0:
+            self.left, self.phase = self.count, self.phase + 1
+
+    def passed(self, parity):
+        return (self.phase & 1) != parity
+
+
+def pair_kernel(stages, parts, runs, rng, free_by_readers):
+    """One pair of thread blocks of ``sq_fp8_pair_kernel`` at the grain of its barriers, its warps stepped in random order:
+    what a drain warp read in place of its run's factors, or None.  ``stages``: of the operand ring; ``parts``: products a
+    run (1: 128 channels, 2: 256).  ``free_by_readers``: a place for factors is free when its readers say so; otherwise
+    when the MMAs of a later run are done."""
+    blocks, depth, drains = (0, 1), 4 // parts, 2
+    full = [Barrier(2) for _ in range(stages)]
+    acc_empty = [Barrier(2 * drains // parts) for _ in range(4)]
+    empty = [[Barrier(parts) for _ in range(stages)] for _ in blocks]
+    acc_full = [[Barrier(1) for _ in range(4)] for _ in blocks]
+    ready = [[Barrier(1) for _ in range(2)] for _ in blocks]
+    free = [[Barrier(drains) for _ in range(2)] for _ in blocks]
+    slots = [[None] * 8 for _ in blocks]
+    wrong = []
+
+    def producer(block):
+        for run in range(runs):
+            yield lambda: empty[block][run % stages].passed((run // stages & 1) ^ 1)
+            full[run % stages].arrive()
+
+    def issuer(mine):
+        for product in range(mine, runs * parts, 2):
+            run, acc = product // parts, product % 4
+            yield lambda: full[run % stages].passed(run // stages & 1)
+            yield lambda: acc_empty[acc].passed((product // 4 & 1) ^ 1)
+            yield lambda: True  # the MMAs end some time after
+            for block in blocks:
+                acc_full[block][acc].arrive()
+                empty[block][run % stages].arrive()
+
+    def factors(block):
+        for batch in range(-(-runs // 4)):
+            if free_by_readers:
+                if batch >= 2:
+                    yield lambda: free[block][batch & 1].passed((batch >> 1 & 1) ^ 1)
+            elif batch:
+                run = 2 if batch == 1 else 4 * batch - 5 + depth
+                yield lambda: empty[block][run % stages].passed(run // stages & 1)
+            for run in range(4 * batch, 4 * batch + 4):
+                slots[block][run & 7] = run
+                yield lambda: True
+            ready[block][batch & 1].arrive()
+
+    def drain(block, share):
+        for run in range(runs):
+            acc = run % 4 if parts == 1 else run * 2 % 4 + share
+            turn = run // 4 if parts == 1 else run // 2
+            yield lambda: acc_full[block][acc].passed(turn & 1)
+            if run % 4 == 0:
+                yield lambda: ready[block][run >> 2 & 1].passed(run >> 3 & 1)
+            if slots[block][run & 7] != run:
+                wrong.append((run, slots[block][run & 7]))
+            acc_empty[acc].arrive()
+            yield lambda: True
+            if run % 4 == 3:
+                free[block][run >> 2 & 1].arrive()
+
+    warps = [producer(0), producer(1), issuer(0), issuer(1), factors(0), factors(1)]
+    warps += [drain(block, share) for block in blocks for share in range(drains)]
+    waiting = {warp: next(warp, None) for warp in warps}
+    pace = {warp: rng.choice((1, 1, 1, 40)) for warp in warps}
+    while any(wait is not None for wait in waiting.values()):
+        able = [warp for warp, wait in waiting.items() if wait is not None and wait()]
+        assert able, "every warp waits"
+        warp = rng.choices(able, [1 / pace[warp] for warp in able])[0]
+        waiting[warp] = next(warp, None)
+        if wrong:
+            return wrong[0]
+    return None
+
+
+@pytest.mark.parametrize("stages,parts", [(7, 1), (5, 2)])
+def test_factors_stay_until_they_are_read(stages, parts):
+    rng = random.Random(stages)
+    for runs in (1, 3, 4, 5, 8, 9, 12, 13, 16, 17, 29, 40, 41):
+        for _ in range(40):
+            assert pair_kernel(stages, parts, runs, rng, free_by_readers=True) is None
+
+
+def test_done_products_do_not_free_factors():
+    """With one product a run, "the MMAs of a later run are done" lets a batch overwrite factors not yet read: the two issuers
+    are not ordered, and a barrier one round behind has the parity waited for.  The stepping above finds it."""
+    rng = random.Random(0)
+    assert any(pair_kernel(7, 1, 40, rng, free_by_readers=False) for _ in range(2000))
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", [(1001, 1480, 2000), (1024, 1408, 14336), (2048, 1024, 4096), (700, 1408, 8208)])
+def test_fp8_gemm_of_128_channel_tiles_and_many_runs(native, quant, m, n, k):
+    """Shapes of the pair kernel with 128 channels a tile and more runs than two batches of factors, back to back."""
+    _, codes, scales, weight, weight_scales, bias = fp8_case(quant, m, n, k, torch.bfloat16)
+    scales = scales * torch.exp2(randn(*scales.shape, seed=9).round())  # every run's factor is another
+    want, size = fp8_product(codes, scales, weight, weight_scales, bias)
+    outs = [native.fp8_gemm(codes, scales, weight, weight_scales, bias, out_dtype=torch.bfloat16) for _ in range(20)]
+    within(outs[0], want, fp8_slack(size, k), torch.bfloat16)
+    assert all(torch.equal(out, outs[0]) for out in outs[1:])
