@@ -38,9 +38,9 @@ struct Device {
   explicit Device(const Tensor& t) : device(t.device()) {
     if (!t.is_cuda() || device.index() != c10::cuda::current_device()) throw No{};
   }
-  // `t` on this device and without a gradient to lose; its address is `align` bytes aligned
+  // `t` on this device and without a gradient or a tangent to lose; its address is `align` bytes aligned
   void* take(const Tensor& t, uintptr_t align) const {
-    if (t.device() != device || (grad && t.requires_grad()) || t.is_conj() || t.is_neg()) throw No{};
+    if (t.device() != device || (grad && t.requires_grad()) || t._fw_grad(0).defined() || t.is_conj() || t.is_neg()) throw No{};
     void* p = t.data_ptr();
     if (reinterpret_cast<uintptr_t>(p) & (align - 1)) throw No{};
     return p;

@@ -5,6 +5,7 @@ graph-private pool, as the reference's ``torch::empty`` calls do,
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -260,12 +261,16 @@ _E4M3 = torch.float8_e4m3fn
 
 
 def _no_gradient(*tensors) -> None:
-    """The operators below are forward only.  An input that autograd tracks is refused: its gradient would be lost
-    without a word."""
+    """The operators below are forward only.  An input that autograd tracks is refused - an e4m3 weight held as a parameter,
+    a forward-mode tangent: its gradient would be lost without a word."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError("the B200 operators have no backward pass: call them under torch.no_grad() or detach the inputs.")
+    if forward_ad._current_level >= 0:  # a dual level is open; no_grad() does not stop tangents
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("the B200 operators have no forward-mode derivative: detach the inputs.")
 
 
 class _Binding:
@@ -395,7 +400,7 @@ def fp8_gemm(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, we
         return y
     if not codes.is_cuda:
         _require_cuda(codes, "codes")
-    _no_gradient(scales, weight_scales, bias, out)
+    _no_gradient(codes, scales, weight, weight_scales, bias, out)
     if codes.dtype is not _E4M3 or codes.ndim < 2:
         raise ValueError("codes must be a float8_e4m3fn tensor with token and channel axes.")
     if out_dtype not in _DTYPES:
@@ -426,7 +431,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tenso
     if out is None and workspace is None and (y := _binding.fp8_linear(x, weight, weight_scales, bias, input_activation)) is not None:
         return y
     _require_rows(x)
-    _no_gradient(x, weight_scales, bias, out)
+    _no_gradient(x, weight, weight_scales, bias, out)
     activation = _input_activation(input_activation)
     device, shape, dtype = x.device, x.shape, x.dtype
     k = shape[-1]

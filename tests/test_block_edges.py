@@ -131,3 +131,48 @@ def test_fp8_gemm_of_128_channel_tiles_and_many_runs(native, quant, m, n, k):
     outs = [native.fp8_gemm(codes, scales, weight, weight_scales, bias, out_dtype=torch.bfloat16) for _ in range(20)]
     within(outs[0], want, fp8_slack(size, k), torch.bfloat16)
     assert all(torch.equal(out, outs[0]) for out in outs[1:])
+
+
+# ---------------------------------------------------------------------------------------------- inputs autograd tracks
+def operator_calls(native, quant, rope):
+    """(name, call, its tensors by name) of each operator on small inputs."""
+    x, codes, scales, weight, weight_scales, bias = fp8_case(quant, 6, 64, 128, torch.bfloat16)
+    linear = dict(weight=weight, weight_scales=weight_scales, bias=bias)
+    vector, rows = randn(128, seed=5), randn(3, 128, seed=6, dtype=torch.bfloat16)
+    norm = dict(x=x, branch=x + 1, gate=rows, post_weight=vector, post_bias=vector, weight=vector, bias=vector, mod_scale=rows, mod_shift=rows)
+    q, k = (randn(1, 6, 2, 64, seed=s, dtype=torch.bfloat16) for s in (7, 8))
+    head = randn(64, seed=9)
+    turn = dict(q=q, k=k, positions=torch.arange(6.0, device="cuda")[:, None], inv_freq=rope.rotary_frequencies((32,), device="cuda"),
+                q_weight=head, k_weight=head)
+    return [("fp8_quantize", lambda t: native.fp8_quantize(t["x"]), dict(x=x)),
+            ("fp8_gemm", lambda t: native.fp8_gemm(**t, out_dtype=torch.bfloat16), dict(codes=codes, scales=scales, **linear)),
+            ("fp8_linear", lambda t: native.fp8_linear(**t), dict(x=x, **linear)),
+            ("block_norm", lambda t: native.block_norm(**t, post_norm="rms"), norm),
+            ("rotary", lambda t: native.rotary(**t, sections=(32,), norm="head"), turn)]
+
+
+@pytest.fixture(scope="module")
+def rope(pkg):
+    return importlib.import_module(P + "rotary")
+
+
+@gpu
+@pytest.mark.parametrize("binding", [True, False])
+def test_every_tracked_input_is_refused(native, quant, rope, binding):
+    native._binding.enabled = binding
+    try:
+        for name, call, tensors in operator_calls(native, quant, rope):
+            call(tensors)
+            for key, tensor in tensors.items():
+                tracked = {**tensors, key: torch.nn.Parameter(tensor)}
+                with pytest.raises(RuntimeError, match="no backward"):
+                    call(tracked)
+                with torch.no_grad():
+                    call(tracked)
+                with torch.autograd.forward_ad.dual_level():
+                    dual = torch.autograd.forward_ad.make_dual(tensor, tensor.clone())
+                    with pytest.raises(RuntimeError, match="no forward-mode"), torch.no_grad():
+                        call({**tensors, key: dual})
+                    call(tensors)
+    finally:
+        native._binding.enabled = True
