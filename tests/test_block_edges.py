@@ -2,11 +2,15 @@
 at the border of what the entry points take, and what they refuse.  Formulas, tolerances and helpers are test_block_ops'."""
 import importlib
 import random
+import re
+from pathlib import Path
 
 import pytest
 import torch
 
 from test_block_ops import DTYPES, P, fp8_case, fp8_product, fp8_slack, gpu, half_step, no_device_timeouts, randn, within  # noqa: F401
+
+ROOT = Path(__file__).resolve().parents[1]
 
 
 @pytest.fixture(scope="module")
@@ -176,3 +180,17 @@ def test_every_tracked_input_is_refused(native, quant, rope, binding):
                     call(tensors)
     finally:
         native._binding.enabled = True
+
+
+# ----------------------------------------------------------------------------------------------- the stack's linears
+@pytest.fixture(scope="module")
+def dit(pkg):
+    return importlib.import_module(P + "dit")
+
+
+def test_configurations_that_users_are_shown(dit):
+    """Every ``DiTConfig(...)`` of the introduction is one."""
+    shown = re.findall(r"DiTConfig\(([^()]*)\)", (ROOT / "README.md").read_text())
+    assert any("rotary=True" in call for call in shown)
+    for call in shown:
+        assert not dit.DiTConfig(**eval(f"dict({call})")).plain
