@@ -148,6 +148,10 @@ class BlockScaledLinear(nn.Module):
         self.dtype, self.backend = weight.dtype, backend
 
     def forward(self, x, *, input_activation: str | None = None) -> torch.Tensor:
+        if input_activation not in (None, "gelu"):
+            raise ValueError("input_activation must be None or 'gelu'.")
+        if isinstance(x, tuple) and (input_activation is not None or self.backend != "native"):
+            raise ValueError("a (codes, scales) pair is quantized already: it takes no input_activation and the native backend.")
         if self.backend == "native":
             if isinstance(x, tuple):
                 return native.fp8_gemm(*x, self.weight, self.weight_scales, self.bias, out_dtype=self.dtype)

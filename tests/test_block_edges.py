@@ -194,3 +194,16 @@ def test_configurations_that_users_are_shown(dit):
     assert any("rotary=True" in call for call in shown)
     for call in shown:
         assert not dit.DiTConfig(**eval(f"dict({call})")).plain
+
+
+def test_a_quantized_input_takes_no_activation(dit):
+    linear = dit.BlockScaledLinear(torch.ones(16, 128), backend="native")
+    pair = (torch.zeros(2, 128).to(torch.float8_e4m3fn), torch.ones(2, 1))
+    with pytest.raises(ValueError, match="no input_activation"):
+        linear(pair, input_activation="gelu")
+    for backend in ("native", "reference"):
+        linear.backend = backend
+        with pytest.raises(ValueError, match="'gelu'"):
+            linear(torch.zeros(2, 128), input_activation="relu")
+    with pytest.raises(ValueError, match="native backend"):
+        linear(pair)
