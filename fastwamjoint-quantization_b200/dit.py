@@ -147,6 +147,15 @@ class BlockScaledLinear(nn.Module):
         self.out_features, self.in_features = weight.shape
         self.dtype, self.backend = weight.dtype, backend
 
+    def _apply(self, fn, recurse=True):
+        """``half()``, ``to(dtype)`` and the like set the type of the output and the bias; the codes and their scales, floating
+        types too, stay what they are and only move."""
+        fixed = {id(self.weight): torch.uint8, id(self.weight_scales): torch.int32}
+        device = self.weight.device
+        super()._apply(lambda t: fn(t.view(fixed[id(t)])).view(t.dtype) if id(t) in fixed else fn(t), recurse)
+        self.dtype = fn(torch.empty(0, dtype=self.dtype, device=device)).dtype
+        return self
+
     def forward(self, x, *, input_activation: str | None = None) -> torch.Tensor:
         if input_activation not in (None, "gelu"):
             raise ValueError("input_activation must be None or 'gelu'.")
@@ -306,6 +315,12 @@ class SyntheticDiT(nn.Module):
             inv_freq = rotary_frequencies(self.sections, device=device)
         self.register_buffer("positions", positions, persistent=False)
         self.register_buffer("inv_freq", inv_freq, persistent=False)
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        if self.inv_freq is not None and self.inv_freq.dtype is not torch.float64:  # to another type: angles stay in 64 bits
+            self.inv_freq = rotary_frequencies(self.sections, device=self.inv_freq.device)
+        return self
 
     def prepack(self) -> "SyntheticDiT":
         """Give every linear a kernel-native copy of its weight (see ``TokenQuantLinear.prepack``)."""

@@ -207,3 +207,39 @@ def test_a_quantized_input_takes_no_activation(dit):
             linear(torch.zeros(2, 128), input_activation="relu")
     with pytest.raises(ValueError, match="native backend"):
         linear(pair)
+
+
+def small_stack(dit, device, **kw):
+    cfg = dit.DiTConfig(**{**dict(blocks=2, hidden=256, heads=2, ffn=256, latent_tokens=12, action_tokens=4, grid=(2, 2, 3), linear="fp8",
+                                  modulated=True, rotary=True), **kw})
+    return dit.SyntheticDiT(cfg, device=device, backend="native" if device == "cuda" else "reference")
+
+
+@pytest.mark.parametrize("move", [lambda m: m.half(), lambda m: m.to(torch.float16), lambda m: m.to("cpu", torch.float16)])
+def test_moving_to_a_dtype_leaves_codes_and_scales(dit, move):
+    linear = dit.BlockScaledLinear(torch.randn(16, 144).bfloat16(), bias=torch.ones(16, dtype=torch.bfloat16), backend="reference")
+    codes, scales, keys = linear.weight.clone(), linear.weight_scales.clone(), list(linear.state_dict())
+    assert move(linear) is linear
+    assert linear.weight.dtype is torch.float8_e4m3fn and torch.equal(linear.weight.view(torch.uint8), codes.view(torch.uint8))
+    assert linear.weight_scales.dtype is torch.float32 and torch.equal(linear.weight_scales, scales)
+    assert list(linear.state_dict()) == keys and linear.bias.dtype is torch.float16
+    assert linear(torch.ones(2, 144)).dtype is torch.float16
+    meta = linear.to("meta")
+    assert meta.weight.is_meta and meta.weight.dtype is torch.float8_e4m3fn and meta.weight_scales.dtype is torch.float32
+    stack = small_stack(dit, "cpu")
+    freq = stack.inv_freq.clone()
+    move(stack)
+    assert torch.equal(stack.inv_freq, freq) and stack.positions.dtype is torch.int32
+
+
+@gpu
+def test_stack_in_half_precision(dit):
+    stack = small_stack(dit, "cuda")
+    x = randn(1, 16, 256)
+    with torch.no_grad():
+        want = stack(x.bfloat16())
+        got = stack.half()(x.half())
+    assert got.dtype is torch.float16
+    # the same weights on inputs and activations rounded to 2^-11 instead of 2^-8: apart by roundings of bf16 and the codes
+    # they flip (the bar of a block's branch in test_block_ops, 4e-2, for each of the two blocks)
+    assert float((got.float() - want.float()).norm() / want.float().norm()) < 8e-2
