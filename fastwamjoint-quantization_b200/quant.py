@@ -81,7 +81,7 @@ def quantize_weight_block(weight: torch.Tensor):
     if weight.ndim != 2:
         raise ValueError("weight must be [N, K].")
     n, k = weight.shape
-    padded = torch.zeros(_blocks(n) * GROUP, _blocks(k) * GROUP, device=weight.device)
+    padded = torch.zeros(_blocks(n) * GROUP, _blocks(k) * GROUP, dtype=torch.float32, device=weight.device)
     padded[:n, :k] = weight.detach().float()
     blocks = padded.view(_blocks(n), GROUP, _blocks(k), GROUP)
     amax = blocks.abs().amax(dim=(1, 3))

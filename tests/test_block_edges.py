@@ -243,3 +243,15 @@ def test_stack_in_half_precision(dit):
     # the same weights on inputs and activations rounded to 2^-11 instead of 2^-8: apart by roundings of bf16 and the codes
     # they flip (the bar of a block's branch in test_block_ops, 4e-2, for each of the two blocks)
     assert float((got.float() - want.float()).norm() / want.float().norm()) < 8e-2
+
+
+def test_weights_quantized_under_another_default_dtype(quant):
+    weight = torch.randn(130, 144)
+    want = quant.quantize_weight_block(weight)
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        got = quant.quantize_weight_block(weight)
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert got[1].dtype is torch.float32 and torch.equal(got[1], want[1])
+    assert torch.equal(got[0].view(torch.uint8), want[0].view(torch.uint8))
