@@ -9,9 +9,12 @@ import ctypes
 import importlib.machinery
 import importlib.util
 import struct
+import warnings
 from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 from functools import lru_cache
 from pathlib import Path
+
+from .build import binding_path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libsq_b200.so"
 
@@ -139,17 +142,21 @@ def load_library() -> ctypes.CDLL:
 
 @lru_cache(maxsize=1)
 def load_binding():
-    """``sq_binding.so`` (``csrc/sq_binding.cpp``), the short way into the library for ordinary calls of the block operators,
-    or None where it has not been built: the ctypes way serves every call."""
-    path = LIB_PATH.with_name("sq_binding.so")
-    if not path.exists():
+    """The binding (``csrc/sq_binding.cpp``), the short way into the library for ordinary calls of the block operators, or None:
+    where none was built for this interpreter and PyTorch, or it does not load, the ctypes way serves every call."""
+    path = binding_path()
+    if path is None or not path.exists():
         return None
     load_library()
     import torch  # noqa: F401  (the module links its libraries)
     loader = importlib.machinery.ExtensionFileLoader("sq_binding", str(path))
     spec = importlib.util.spec_from_file_location("sq_binding", str(path), loader=loader)
-    module = importlib.util.module_from_spec(spec)
-    loader.exec_module(module)
+    try:
+        module = importlib.util.module_from_spec(spec)
+        loader.exec_module(module)
+    except ImportError as error:
+        warnings.warn(f"{path.name} does not load, the block operators' calls go through ctypes: {error}")
+        return None
     return module
 
 

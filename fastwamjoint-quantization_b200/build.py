@@ -6,26 +6,28 @@ The library has a C ABI only (``include/sq_b200.h``); it links the CUDA runtime
 statically and needs neither PyTorch nor libcuda at link time (the one driver
 call it makes, ``cuTensorMapEncodeTiled``, is looked up at run time).
 
-Beside it goes ``sq_binding.so``, a small CPython module over that C ABI which takes the
+Beside it goes ``sq_binding``, a small CPython module over that C ABI which takes the
 block operators' ordinary calls (``csrc/sq_binding.cpp``); it is compiled by the host
-compiler against PyTorch's headers.
+compiler against PyTorch's headers.  It is optional: where it cannot be built there is a
+warning, and the calls go through ctypes.
 """
 from __future__ import annotations
 
 import argparse
 import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 LIB = HERE / "lib" / "libsq_b200.so"
-BINDING = HERE / "lib" / "sq_binding.so"
 BINDING_SOURCE = CSRC / "sq_binding.cpp"
 SOURCES = ("sq_prepass.cu", "sq_gemm_tc.cu", "sq_gemm_ts.cu", "sq_fp8_gemm.cu", "sq_block_norm.cu", "sq_rotary.cu",
            "sq_api.cu")
@@ -49,18 +51,30 @@ def stale() -> bool:
     return any(d.stat().st_mtime > built for d in deps)
 
 
-def build_binding(force: bool = False, verbose: bool = False) -> Path:
-    """``sq_binding.so``, linked against the built library (found beside it at run time) and PyTorch's own."""
-    deps = [BINDING_SOURCE, (CSRC / "../../include/sq_b200.h").resolve(), Path(__file__)]
-    if not force and BINDING.exists() and all(d.stat().st_mtime <= BINDING.stat().st_mtime for d in deps):
-        return BINDING
+def binding_path() -> Path | None:
+    """Where the binding for this interpreter and this PyTorch lies, or None without a PyTorch.  The module reads C++ objects
+    of both, so its name says which it was compiled against: another release finds no module, not a wrong one."""
     spec = importlib.util.find_spec("torch")
-    compiler = shutil.which("g++")
-    if spec is None or compiler is None:
-        raise RuntimeError("PyTorch and g++ are needed to build sq_binding.so.")
-    torch_dir = Path(spec.origin).parent
+    version = Path(spec.origin).with_name("version.py") if spec is not None and spec.origin else None
+    found = re.search(r"^__version__ = '([^']+)'", version.read_text(), re.M) if version is not None and version.exists() else None
+    if found is None:
+        return None
+    return LIB.with_name(f"sq_binding.{sysconfig.get_config_var('SOABI')}.torch-{found[1]}.so")
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> Path | None:
+    """The binding, linked against the built library (found beside it at run time) and PyTorch's own; None, with a warning,
+    where it cannot be built."""
+    binding, compiler = binding_path(), shutil.which("g++")
+    if binding is None or compiler is None:
+        warnings.warn("sq_binding needs PyTorch and g++ to be built; the block operators' calls go through ctypes.")
+        return None
+    deps = [BINDING_SOURCE, (CSRC / "../../include/sq_b200.h").resolve(), Path(__file__)]
+    if not force and binding.exists() and all(d.stat().st_mtime <= binding.stat().st_mtime for d in deps):
+        return binding
+    torch_dir = Path(importlib.util.find_spec("torch").origin).parent
     cuda = Path(nvcc()).resolve().parents[1]
-    tmp = BINDING.with_suffix(".so.tmp")
+    tmp = binding.with_suffix(".so.tmp")
     cmd = [compiler, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-isystem", str(torch_dir / "include"),
            "-isystem", str(torch_dir / "include/torch/csrc/api/include"), "-isystem", str(cuda / "include"),
            "-I", sysconfig.get_paths()["include"], str(BINDING_SOURCE), "-o", str(tmp), f"-L{LIB.parent}", f"-l:{LIB.name}",
@@ -69,9 +83,11 @@ def build_binding(force: bool = False, verbose: bool = False) -> Path:
     if verbose or done.returncode:
         sys.stderr.write(done.stdout + done.stderr)
     if done.returncode:
-        raise RuntimeError("building sq_binding.so failed")
-    os.replace(tmp, BINDING)
-    return BINDING
+        binding.unlink(missing_ok=True)  # of older sources
+        warnings.warn("building sq_binding failed; the block operators' calls go through ctypes.")
+        return None
+    os.replace(tmp, binding)
+    return binding
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:

@@ -255,3 +255,30 @@ def test_weights_quantized_under_another_default_dtype(quant):
         torch.set_default_dtype(torch.float32)
     assert got[1].dtype is torch.float32 and torch.equal(got[1], want[1])
     assert torch.equal(got[0].view(torch.uint8), want[0].view(torch.uint8))
+
+
+# -------------------------------------------------------------------------------------------- the binding is optional
+def test_building_without_a_host_compiler_or_pytorch(pkg, monkeypatch):
+    build = importlib.import_module(P + "build")
+    monkeypatch.setattr(build, "stale", lambda: False)
+    which = build.shutil.which
+    monkeypatch.setattr(build.shutil, "which", lambda name: None if name == "g++" else which(name))
+    with pytest.warns(UserWarning, match="needs PyTorch and g"):
+        assert build.build() == build.LIB
+    monkeypatch.setattr(build.shutil, "which", which)
+    monkeypatch.setattr(build, "binding_path", lambda: None)
+    with pytest.warns(UserWarning, match="needs PyTorch and g"):
+        assert build.build() == build.LIB
+
+
+def test_binding_of_another_release_or_broken(pkg, monkeypatch, tmp_path):
+    lib, build = importlib.import_module(P + "_lib"), importlib.import_module(P + "build")
+    assert f"torch-{torch.__version__}.so" in build.binding_path().name and "cpython" in build.binding_path().name
+    load = lib.load_binding.__wrapped__
+    monkeypatch.setattr(lib, "binding_path", lambda: tmp_path / "sq_binding.of-another-release.so")
+    assert load() is None
+    (tmp_path / "sq_binding.of-another-release.so").write_bytes(b"not a shared object")
+    with pytest.warns(UserWarning, match="does not load"):
+        assert load() is None
+    monkeypatch.setattr(lib, "binding_path", lambda: None)
+    assert load() is None
