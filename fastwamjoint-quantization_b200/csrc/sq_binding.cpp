@@ -77,6 +77,18 @@ void need(bool ok) {
   if (!ok) throw No{};
 }
 
+// Allocation may wait for the device and a launch for room in its queue: other Python threads run meanwhile.
+class NoLock {
+ public:
+  NoLock() : state_(PyEval_SaveThread()) {}
+  ~NoLock() { PyEval_RestoreThread(state_); }
+  NoLock(const NoLock&) = delete;
+  NoLock& operator=(const NoLock&) = delete;
+
+ private:
+  PyThreadState* state_;
+};
+
 PyObject* wrap(Tensor t) { return THPVariable_Wrap(std::move(t)); }
 
 struct Weight {
@@ -119,9 +131,13 @@ PyObject* gemm(PyObject* const* a) {
   const int64_t rows = x.numel() / w.k;
   need(s.scalar_type() == at::kFloat && s.dim() == 2 && s.size(0) == rows && s.size(1) == (w.k + 127) / 128);
   const float* scales = static_cast<const float*>(d.take(s, 4));
-  Tensor out = output_like(x, w.n, out_type);
-  need(sq_fp8_gemm(codes, scales, s.stride(0), s.stride(1), w.codes, w.scales, w.bias, out.data_ptr(),
-                   out_type == at::kBFloat16 ? SQ_BF16 : SQ_FP16, rows, w.n, w.k, d.stream()) == SQ_OK);
+  Tensor out;
+  {
+    const NoLock released;
+    out = output_like(x, w.n, out_type);
+    need(sq_fp8_gemm(codes, scales, s.stride(0), s.stride(1), w.codes, w.scales, w.bias, out.data_ptr(),
+                     out_type == at::kBFloat16 ? SQ_BF16 : SQ_FP16, rows, w.n, w.k, d.stream()) == SQ_OK);
+  }
   return wrap(std::move(out));
 }
 
@@ -136,10 +152,14 @@ PyObject* linear(PyObject* const* a) {
   need(x.size(-1) == w.k && x.numel() > 0);
   const int64_t rows = x.numel() / w.k;
   const size_t bytes = sq_fp8_workspace_bytes(rows, w.k);
-  Tensor workspace = at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte));
-  Tensor out = output_like(x, w.n, x.scalar_type());
-  need(sq_fp8_linear(from, dtype, rows, w.k, w.n, activation, w.codes, w.scales, w.bias, out.data_ptr(), workspace.data_ptr(),
-                     bytes, d.stream()) == SQ_OK);
+  Tensor out;
+  {
+    const NoLock released;
+    const Tensor workspace = at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte));
+    out = output_like(x, w.n, x.scalar_type());
+    need(sq_fp8_linear(from, dtype, rows, w.k, w.n, activation, w.codes, w.scales, w.bias, out.data_ptr(), workspace.data_ptr(),
+                       bytes, d.stream()) == SQ_OK);
+  }
   return wrap(std::move(out));
 }
 
@@ -203,25 +223,30 @@ PyObject* block_norm(PyObject* const* a) {
   b.bias = channel_param(d, a[9], x);
   b.mod_scale = rows_param(d, a[10], x, b.rows);
   b.mod_shift = rows_param(d, a[11], x, b.rows);
-  Tensor h, z, scales;
   if (branch) {
     const Tensor& t = tensor_of(a[1]);
     need(t.scalar_type() == x.scalar_type() && t.sizes() == x.sizes() && t.is_contiguous());
     b.branch = d.take(t, 16);
-    h = at::empty(x.sizes(), x.options());
-    b.h_out = h.data_ptr();
   }
-  if (b.norm_kind != SQ_NORM_NONE) {
-    z = at::empty(x.sizes(), x.options().dtype(quantize ? at::kFloat8_e4m3fn : x.scalar_type()));
-    b.z_out = z.data_ptr();
-    if (quantize) {
-      scales = at::empty_strided({b.rows, (b.width + 127) / 128}, {1, b.rows}, x.options().dtype(at::kFloat));
-      b.scales = scales.data_ptr<float>();
-      b.scales_row_stride = 1;
-      b.scales_group_stride = b.rows;
+  Tensor h, z, scales;
+  {
+    const NoLock released;
+    if (branch) {
+      h = at::empty(x.sizes(), x.options());
+      b.h_out = h.data_ptr();
     }
+    if (b.norm_kind != SQ_NORM_NONE) {
+      z = at::empty(x.sizes(), x.options().dtype(quantize ? at::kFloat8_e4m3fn : x.scalar_type()));
+      b.z_out = z.data_ptr();
+      if (quantize) {
+        scales = at::empty_strided({b.rows, (b.width + 127) / 128}, {1, b.rows}, x.options().dtype(at::kFloat));
+        b.scales = scales.data_ptr<float>();
+        b.scales_row_stride = 1;
+        b.scales_group_stride = b.rows;
+      }
+    }
+    need(sq_block_norm(&b, d.stream()) == SQ_OK);
   }
-  need(sq_block_norm(&b, d.stream()) == SQ_OK);
   PyObject* first = a[0];
   if (branch) first = wrap(std::move(h));
   else Py_INCREF(first);
@@ -291,8 +316,6 @@ PyObject* rotary(PyObject* const* a) {
   r.position_batch_stride = pd == 3 && positions.size(0) > 1 ? positions.stride(0) : 0;
   r.eps = static_cast<float>(number(a[9]));
   r.q_weight = rotary_weight(d, a[7], q, r.heads, r.norm, &r.q_weight_fp32);
-  Tensor q_out = at::empty(q.sizes(), q.options()), k_out;
-  r.q_out = q_out.data_ptr();
   auto dense = [&](int64_t heads, int64_t (&s)[3]) {
     s[2] = r.dim;
     s[1] = heads * r.dim;
@@ -308,8 +331,6 @@ PyObject* rotary(PyObject* const* a) {
     std::memcpy(r.k_strides, kh.strides, sizeof(kh.strides));
     r.kv_heads = static_cast<int32_t>(k.size(2));
     r.k_weight = rotary_weight(d, a[8], q, r.kv_heads, r.norm, &r.k_weight_fp32);
-    k_out = at::empty(k.sizes(), k.options());
-    r.k_out = k_out.data_ptr();
     dense(r.kv_heads, r.k_out_strides);
   } else {
     need(a[8] == Py_None);
@@ -317,7 +338,17 @@ PyObject* rotary(PyObject* const* a) {
   int64_t lanes = 1;
   while (8 * lanes < r.dim) lanes *= 2;
   need((r.heads + static_cast<int64_t>(r.kv_heads)) * lanes <= 4096);
-  need(sq_rotary(&r, d.stream()) == SQ_OK);
+  Tensor q_out, k_out;
+  {
+    const NoLock released;
+    q_out = at::empty(q.sizes(), q.options());
+    r.q_out = q_out.data_ptr();
+    if (a[1] != Py_None) {
+      k_out = at::empty({r.batch, r.length, r.kv_heads, r.dim}, q.options());
+      r.k_out = k_out.data_ptr();
+    }
+    need(sq_rotary(&r, d.stream()) == SQ_OK);
+  }
   PyObject* second = Py_None;
   if (a[1] != Py_None) second = wrap(std::move(k_out));
   else Py_INCREF(second);

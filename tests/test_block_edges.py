@@ -3,6 +3,8 @@ at the border of what the entry points take, and what they refuse.  Formulas, to
 import importlib
 import random
 import re
+import threading
+import time
 from pathlib import Path
 
 import pytest
@@ -282,3 +284,57 @@ def test_binding_of_another_release_or_broken(pkg, monkeypatch, tmp_path):
         assert load() is None
     monkeypatch.setattr(lib, "binding_path", lambda: None)
     assert load() is None
+
+
+# ------------------------------------------------------------------------------------------------------ host threads
+@gpu
+def test_other_threads_run_while_a_call_waits(native):
+    """A call that waits for room in the launch queue does not hold the interpreter: a thread that ticks every millisecond
+    goes on while the device is busy for about half a second and more launches are asked for than its queue holds."""
+    x = randn(64, 1024, dtype=torch.bfloat16)
+    native.block_norm(x)
+    torch.cuda.synchronize()
+    ticks, done = [], threading.Event()
+
+    def tick():
+        while not done.wait(0.001):
+            ticks.append(time.perf_counter())
+
+    thread = threading.Thread(target=tick)
+    thread.start()
+    try:
+        torch.cuda._sleep(10 ** 9)
+        begin = time.perf_counter()
+        for _ in range(3000):
+            native.block_norm(x)
+        waited = time.perf_counter() - begin
+    finally:
+        done.set()
+        thread.join()
+    torch.cuda.synchronize()
+    assert waited > 0.2, "the launches did not wait for the device"
+    longest = max(b - a for a, b in zip(ticks, ticks[1:]))
+    assert longest < waited / 4
+
+
+@gpu
+def test_calls_from_two_threads(native, quant):
+    x, _, _, weight, weight_scales, bias = fp8_case(quant, 300, 512, 1024, torch.bfloat16)
+    want, want_norm = native.fp8_linear(x, weight, weight_scales, bias), native.block_norm(x, x)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                y, (h, z) = native.fp8_linear(x, weight, weight_scales, bias), native.block_norm(x, x)
+                torch.cuda.current_stream().synchronize()
+                if not (torch.equal(y, want) and torch.equal(h, want_norm[0]) and torch.equal(z, want_norm[1])):
+                    wrong.append(1)
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not wrong
