@@ -21,6 +21,7 @@ LIB_PATH = Path(__file__).resolve().parent / "lib" / "libsq_b200.so"
 # status codes of include/sq_b200.h
 OK, ERR_NULL, ERR_SHAPE, ERR_ENUM, ERR_INDEX, ERR_DRIVER, ERR_WORKSPACE, ERR_DEVICE_WAIT = 0, -1, -2, -3, -4, -5, -6, -7
 ERR_SCRATCH_LIMIT = -8
+ERR_OVERLAP = -9
 NOALLOC_SCRATCH_BYTES = 8 * 1024 * 1024 + 65536
 BF16, FP16 = 0, 1
 ACT_STATIC, ACT_TOKEN = 0, 1
@@ -167,6 +168,9 @@ def status_string(status: int) -> str:
 def check(status: int, what: str) -> None:
     """Turn a non-zero status into the exception type the reference raises at the
     same place: argument errors found by its C++ checks are RuntimeError
-    (TORCH_CHECK, kernels/w4a8/csrc/w4a8.cu:1079-1115)."""
+    (TORCH_CHECK, kernels/w4a8/csrc/w4a8.cu:1079-1115).  Overlap, which only the block
+    operators look for, is a ValueError like their other refusals."""
+    if status == ERR_OVERLAP:
+        raise ValueError(f"{what}: {status_string(status)}.")
     if status != OK:
         raise RuntimeError(f"{what}: {status_string(status)} (status {status})")

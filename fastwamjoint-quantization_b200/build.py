@@ -31,7 +31,7 @@ LIB = HERE / "lib" / "libsq_b200.so"
 BINDING_SOURCE = CSRC / "sq_binding.cpp"
 SOURCES = ("sq_prepass.cu", "sq_gemm_tc.cu", "sq_gemm_ts.cu", "sq_fp8_gemm.cu", "sq_block_norm.cu", "sq_rotary.cu",
            "sq_api.cu")
-HEADERS = ("sq_internal.h", "sq_ptx.cuh", "sq_rows.cuh", "../../include/sq_b200.h")
+HEADERS = ("sq_internal.h", "sq_overlap.h", "sq_ptx.cuh", "sq_rows.cuh", "../../include/sq_b200.h")
 NVCC_FLAGS = ("-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden")
 

@@ -10,6 +10,7 @@
 #include <type_traits>
 
 #include "sq_internal.h"
+#include "sq_overlap.h"
 
 namespace sq {
 
@@ -356,6 +357,9 @@ int sq_fp8_linear(const void* x, int x_dtype, int64_t rows, int64_t K, int64_t N
   sq::Fp8GemmArgs gemm = {workspace, scales, 1, rows, weight, weight_scales, bias, out, x_dtype, rows, N, K, true};
   const int refused = sq::validate_fp8_gemm(gemm);  // before the quantizer: a refused call launches nothing
   if (refused != SQ_OK || rows == 0) return refused;
+  const int64_t runs = (K + 127) / 128;
+  for (const sq::View& read : {sq::View(weight, N * K), sq::View(weight_scales, 4 * runs * ((N + 127) / 128)), sq::View(bias, 2 * N)})
+    if (sq::overlaps(sq::View(workspace, static_cast<int64_t>(sq_fp8_workspace_bytes(rows, K))), read)) return SQ_ERR_OVERLAP;
   const int status = sq::launch_fp8_quantize(x, x_dtype, rows, K, input_activation, workspace, scales, 1, rows,
                                              static_cast<cudaStream_t>(stream));
   return status != SQ_OK ? status : sq::launch_fp8_gemm(gemm, static_cast<cudaStream_t>(stream));
@@ -559,6 +563,7 @@ const char* sq_status_string(int status) {
     case SQ_ERR_DRIVER: return "CUDA driver call failed";
     case SQ_ERR_WORKSPACE: return "workspace too small";
     case SQ_ERR_DEVICE_WAIT: return "a kernel gave up a bounded wait";
+    case SQ_ERR_OVERLAP: return "an output must share no memory with itself, an input or another output, except where it may be an input itself";
     case SQ_ERR_SCRATCH_LIMIT: return "rows * K is beyond the library-owned scratch of sq_linear_noalloc";
     case 9006: return "device: the MMA rate probe timed out waiting for its MMAs";
     case 9007: return "device: drain warp timed out waiting for its partner at a block of group scales";

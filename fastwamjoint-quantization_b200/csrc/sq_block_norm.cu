@@ -11,6 +11,7 @@
 #include <type_traits>
 
 #include "sq_internal.h"
+#include "sq_overlap.h"
 #include "sq_rows.cuh"
 
 namespace sq {
@@ -319,6 +320,9 @@ int launch_fp8_quantize(const void* x, int x_dtype, int64_t rows, int64_t K, int
   if (rows == 0) return SQ_OK;
   const int64_t per_row = (K + 127) / 128;
   if (rows > (int64_t{1} << 30) / per_row) return SQ_ERR_SHAPE;
+  if (scales_row < 0 || scales_group < 0) return SQ_ERR_SHAPE;
+  const View from(x, rows * K * 2), to(codes, rows * K), scale_view(scales, 4, rows, scales_row * 4, per_row, scales_group * 4);
+  if (clashes(to, {from, scale_view}) || clashes(scale_view, {from})) return SQ_ERR_OVERLAP;
   const uint32_t runs = static_cast<uint32_t>(rows * per_row);
   const Divisor by = divisor(per_row);
   const unsigned blocks = (runs + kQuantThreads / 16 * kRuns - 1) / (kQuantThreads / 16 * kRuns);
@@ -333,6 +337,28 @@ int launch_fp8_quantize(const void* x, int x_dtype, int64_t rows, int64_t K, int
   else gelu ? go(__half{}, std::true_type{}) : go(__half{}, std::false_type{});
   const cudaError_t err = cudaGetLastError();
   return err == cudaSuccess ? SQ_OK : static_cast<int>(err);
+}
+
+// h and z may take the place of x or branch, row by row; else what is written shares memory with nothing.
+static int norm_overlap(const SqBlockNorm& b) {
+  const int64_t bytes = b.rows * b.width;
+  const View x(b.x, 2 * bytes), branch(b.branch, 2 * bytes);
+  const View h(b.branch != nullptr ? b.h_out : nullptr, 2 * bytes);
+  const View z(b.norm_kind != SQ_NORM_NONE ? b.z_out : nullptr, b.scales != nullptr ? bytes : 2 * bytes);
+  const View scales(b.scales, 4, b.rows, 4 * b.scales_row_stride, (b.width + 127) / 128, 4 * b.scales_group_stride);
+  auto channels = [&](const SqParam& q) { return View(q.data, b.width * (q.is_fp32 ? 4 : 2)); };
+  auto table = [&](const SqParam& q) {
+    const int64_t size = q.is_fp32 ? 4 : 2, groups = q.data == nullptr || q.span <= 0 ? 1 : (b.rows + q.span - 1) / q.span;
+    return View(q.data, b.width * size, groups, q.row_stride * size);
+  };
+  for (const View& out : {h, z, scales}) {
+    if (clashes(out, {channels(b.post_weight), channels(b.post_bias), channels(b.weight), channels(b.bias), table(b.gate),
+                      table(b.mod_scale), table(b.mod_shift)}))
+      return SQ_ERR_OVERLAP;
+    for (const View& in : {x, branch})
+      if (!same_view(out, in) && overlaps(out, in)) return SQ_ERR_OVERLAP;
+  }
+  return overlaps(h, z) || overlaps(h, scales) || overlaps(z, scales) ? SQ_ERR_OVERLAP : SQ_OK;
 }
 
 int launch_block_norm(const SqBlockNorm& b, cudaStream_t stream) {
@@ -371,7 +397,10 @@ int launch_block_norm(const SqBlockNorm& b, cudaStream_t stream) {
   a.mod_shift = take(b.mod_shift);
   for (const Param& q : {a.gate, a.post_weight, a.post_bias, a.weight, a.bias, a.mod_scale, a.mod_shift})
     if (!aligned_param_host(q.p, q.f32 != 0)) return SQ_ERR_SHAPE;
+  if (b.scales != nullptr && (b.scales_row_stride < 0 || b.scales_group_stride < 0)) return SQ_ERR_SHAPE;
   if (b.rows == 0) return SQ_OK;
+  const int overlap = norm_overlap(b);
+  if (overlap != SQ_OK) return overlap;
   a.x = b.x;
   a.branch = b.branch;
   a.residual_scale = b.residual_scale;

@@ -20,6 +20,7 @@
 #include <mutex>
 
 #include "sq_internal.h"
+#include "sq_overlap.h"
 #include "sq_ptx.cuh"
 #include "sq_rows.cuh"
 
@@ -964,6 +965,11 @@ int validate_fp8_gemm(const Fp8GemmArgs& a) {
   if (((reinterpret_cast<uintptr_t>(a.scales) | reinterpret_cast<uintptr_t>(a.weight_scales)) & 3u) != 0) return SQ_ERR_SHAPE;
   if ((reinterpret_cast<uintptr_t>(a.bias) & 1u) != 0) return SQ_ERR_SHAPE;
   if (a.scales_row < 0 || a.scales_group < 0) return SQ_ERR_SHAPE;
+  const int64_t runs = (a.K + kRun - 1) / kRun;
+  if (clashes(View(a.out, 2 * a.M * a.N),
+              {View(a.codes, a.M * a.K), View(a.scales, 4, a.M, 4 * a.scales_row, runs, 4 * a.scales_group), View(a.weight, a.N * a.K),
+               View(a.weight_scales, 4 * runs * ((a.N + kRun - 1) / kRun)), View(a.bias, 2 * a.N)}))
+    return SQ_ERR_OVERLAP;
   return SQ_OK;
 }
 

@@ -16,6 +16,7 @@
 // lane's loads of several heads are issued before the first is used.  The norm over a token's heads reads a token that does
 // not fit its block's registers twice, the second time out of the L1.
 #include "sq_internal.h"
+#include "sq_overlap.h"
 #include "sq_rows.cuh"
 
 namespace sq {
@@ -437,6 +438,24 @@ int launch_typed(const RotaryArgs& a, int64_t batch, int layout, int norm, cudaS
 
 }  // namespace
 
+// q_out may be q and k_out may be k, index by index; else what is written shares memory with nothing.
+static int rotary_overlap(const SqRotary& r, int pairs) {
+  auto heads = [&](const void* at, int32_t count, const int64_t (&s)[3]) {
+    return View(at, 2 * r.dim, r.batch, 2 * s[0], r.length, 2 * s[1], count, 2 * s[2]);
+  };
+  const View q = heads(r.q, r.heads, r.q_strides), q_out = heads(r.q_out, r.heads, r.q_out_strides);
+  const View k = heads(r.k, r.kv_heads, r.k_strides), k_out = heads(r.k_out, r.kv_heads, r.k_out_strides);
+  const int token = r.norm == SQ_ROTARY_NORM_TOKEN, size = r.position_type == SQ_POS_INT64 ? 8 : 4;
+  const View q_weight(r.q_weight, (r.q_weight_fp32 ? 4 : 2) * r.dim * (token ? r.heads : 1));
+  const View k_weight(r.k_weight, (r.k_weight_fp32 ? 4 : 2) * r.dim * (token ? r.kv_heads : 1));
+  const View positions(r.positions, size * r.axes, r.batch, size * r.position_batch_stride, r.length, size * r.position_token_stride);
+  const View inv_freq(r.inv_freq, 8 * pairs);
+  for (const View& out : {q_out, k_out})
+    if (clashes(out, {q_weight, k_weight, positions, inv_freq})) return SQ_ERR_OVERLAP;
+  if ((!same_view(q_out, q) && overlaps(q_out, q)) || (!same_view(k_out, k) && overlaps(k_out, k))) return SQ_ERR_OVERLAP;
+  return overlaps(q_out, k) || overlaps(k_out, q) || overlaps(q_out, k_out) ? SQ_ERR_OVERLAP : SQ_OK;
+}
+
 int launch_rotary(const SqRotary& r, cudaStream_t stream) {
   if (r.q == nullptr || r.q_out == nullptr || r.positions == nullptr || r.inv_freq == nullptr) return SQ_ERR_NULL;
   if (r.kv_heads > 0 && (r.k == nullptr || r.k_out == nullptr)) return SQ_ERR_NULL;
@@ -474,6 +493,8 @@ int launch_rotary(const SqRotary& r, cudaStream_t stream) {
   if ((reinterpret_cast<uintptr_t>(r.inv_freq) & 7u) != 0) return SQ_ERR_SHAPE;
   if (r.batch > 0 && r.length > (int64_t{1} << 40) / r.batch) return SQ_ERR_SHAPE;
   if (r.batch * r.length == 0) return SQ_OK;
+  const int overlap = rotary_overlap(r, end);
+  if (overlap != SQ_OK) return overlap;
   a.q = r.q;
   a.k = r.k;
   a.q_out = r.q_out;

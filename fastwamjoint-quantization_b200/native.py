@@ -395,7 +395,8 @@ def fp8_gemm(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, we
              out_dtype: torch.dtype, out: torch.Tensor | None = None) -> torch.Tensor:
     """e4m3 codes [..., K] (with fp32 ``scales`` [rows, ceil(K / 128)], any strides) x e4m3 weight [N, K] (with fp32
     ``weight_scales`` [ceil(N / 128), ceil(K / 128)], one per 128 x 128 block) + bias -> [..., N] in ``out_dtype``.  Sums in
-    fp32, one rounding.  ``quant.quantize_weight_block`` makes the weight's form, ``fp8_quantize`` the codes'."""
+    fp32, one rounding.  ``quant.quantize_weight_block`` makes the weight's form, ``fp8_quantize`` the codes'.  ``out`` shares no
+    memory with an input (refused)."""
     if out is None and (y := _binding.fp8_gemm(codes, scales, weight, weight_scales, bias, out_dtype)) is not None:
         return y
     if not codes.is_cuda:
@@ -427,7 +428,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tenso
                workspace: torch.Tensor | None = None) -> torch.Tensor:
     """``linear([gelu](x))`` in e4m3: ``fp8_quantize`` and ``fp8_gemm`` as one call, the product's set-up and first weight
     loads running under the quantizer.  ``workspace`` (uint8, at least ``sq_fp8_workspace_bytes(rows, K)``) may be passed
-    to reuse a buffer across calls that are ordered on the device."""
+    to reuse a buffer across calls that are ordered on the device; ``out`` may be x's memory, but share none with the others."""
     if out is None and workspace is None and (y := _binding.fp8_linear(x, weight, weight_scales, bias, input_activation)) is not None:
         return y
     _require_rows(x)
@@ -451,19 +452,6 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tenso
         _call("sq_fp8_linear", device, x.data_ptr(), _DTYPES[dtype], rows, k, n, activation, weight.data_ptr(),
               weight_scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), workspace.data_ptr(), nbytes)
     return out
-
-
-def _refuse_overlap(out: torch.Tensor, same, others) -> None:
-    """``out`` is written while other rows are still read: it may be one of ``same`` itself, but share no memory with them or
-    with ``others`` otherwise."""
-    begin = out.data_ptr()
-    end = begin + out.numel() * out.element_size()
-    for t in (*(t for t in same if t.data_ptr() != begin), *others):
-        if t is None or t.numel() == 0:
-            continue
-        at = t.data_ptr()
-        if at < end and begin < at + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size():
-            raise ValueError("out must be x or branch itself, or share no memory with the inputs.")
 
 
 _ABSENT = (0, 0, 0, 0, 0)
@@ -527,7 +515,7 @@ def block_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *, gate=None
     [width]; gate, mod_scale and mod_shift [..., width], each row for an equal share of x's rows (a strided slice of a
     modulation table is read in place), all in x's dtype or fp32.  ``quantize`` gives z as ``(codes, scales)`` for
     ``fp8_gemm`` (``fp8_quantize``'s rule, no rounding to x's dtype between).  ``out`` takes h; it may be x or branch itself,
-    and shares no memory with an input otherwise."""
+    and shares no memory with an input otherwise (refused)."""
     if out is None and (pair := _binding.block_norm(x, branch, gate, residual_scale, post_norm, post_weight, post_bias, norm,
                                                          weight, bias, mod_scale, mod_shift, eps, quantize)) is not None:
         return pair
@@ -548,7 +536,6 @@ def block_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *, gate=None
     x_rows = _vectors(x)
     rows = x.numel() // width
     kept = []  # copies made for alignment live until the launch
-    parameters = (gate, post_weight, post_bias, weight, bias, mod_scale, mod_shift)
     gate, mod_scale, mod_shift = (_row_param(t, kept, rows, width, dtype, device, name) for t, name in (
         (gate, "gate"), (mod_scale, "mod_scale"), (mod_shift, "mod_shift")))
     post_weight, post_bias, weight, bias = (_channel_param(t, kept, width, dtype, device, name) for t, name in (
@@ -563,7 +550,6 @@ def block_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *, gate=None
             h = torch.empty_like(x_rows)
         else:
             h = _checked_output(out, shape, dtype, device)
-            _refuse_overlap(h, (x_rows, branch), parameters)
         branch_ptr, h_ptr = branch.data_ptr(), h.data_ptr()
     if norm is not None:
         z = torch.empty_like(x_rows, dtype=_E4M3) if quantize else torch.empty_like(x_rows)
@@ -638,8 +624,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     ``-positions`` undoes it).  ``layout``: pairs are neighbours ("interleaved") or half the rotated length apart
     ("half"); elements past 2 * pairs pass through.  ``norm``: RMS of each head ("head", weights [dim]) or over all
     heads of a token ("token", weights [heads * dim]), statistics in fp32 (values up to 2^59).  ``out`` is a pair (q, k) of
-    tensors to write, strided as a cache or a transposed view may be; they may be the inputs themselves, but overlap
-    nothing otherwise."""
+    tensors to write, strided as a cache or a transposed view may be; they may be the inputs themselves, and share
+    no memory with an input, each other or themselves otherwise (refused)."""
     if out is None and (pair := _binding.rotary(q, k, positions, inv_freq, sections, layout, norm, q_weight, k_weight, eps)) is not None:
         return pair
     if not q.is_cuda:

@@ -32,6 +32,7 @@ extern "C" {
 #define SQ_ERR_WORKSPACE (-6) /* workspace smaller than sq_workspace_bytes()           */
 #define SQ_ERR_DEVICE_WAIT (-7) /* a kernel gave up a bounded wait (see sq_device_status) */
 #define SQ_ERR_SCRATCH_LIMIT (-8) /* sq_linear_noalloc: the linear needs more scratch than the library owns */
+#define SQ_ERR_OVERLAP (-9)   /* an output shares memory with itself, an input or another output (block operators) */
 
 /* element types of activations / outputs */
 #define SQ_BF16 0
@@ -286,7 +287,9 @@ int sq_linear_noalloc(const void* x, int x_dtype, int64_t rows, int64_t K, int64
                       const void* w_packed, const void* w_scales, int wscale_mode, const void* bias,
                       void* out, void* stream);
 
-/* ---- Operators of a transformer block beside the int4 linears (no counterpart in the reference) ---- */
+/* ---- Operators of a transformer block beside the int4 linears (no counterpart in the reference) ----
+ * What they write shares no memory with what they read or write beside it (SQ_ERR_OVERLAP), except where a function says
+ * that an output may be an input itself: the same address and strides. */
 
 /* Activations to e4m3: x [rows, K] bf16 / fp16 (x_dtype) -> codes [rows, K] and one fp32 scale per row and run of 128 k
  * (the last run may be shorter): scale = max(amax / 448, 1e-8), code = e4m3(x * (1 / scale)), round to nearest even,
@@ -324,7 +327,7 @@ typedef struct SqParam {
 /* The norms before and after a block with its gate and residual scale:
  *   b = post(branch) * post_weight + post_bias
  *   h = residual_scale * x + gate * b                      -> h_out, in x's type (may be x or branch itself)
- *   z = (norm(h) * weight + bias) * (1 + mod_scale) + mod_shift  -> z_out
+ *   z = (norm(h) * weight + bias) * (1 + mod_scale) + mod_shift  -> z_out (without scales: the same, but not h_out)
  * post_kind / norm_kind: SQ_NORM_NONE, SQ_NORM_LAYER or SQ_NORM_RMS over the row, fp32 statistics of the unrounded h.
  * branch null: h is x, nothing is written to h_out.  norm_kind none: only h.  scales null: z in x's type; else z_out takes
  * e4m3 codes and scales one fp32 per row and run of 128 (sq_fp8_quantize's rule).  width % 8 == 0 (16 with scales),

@@ -1,8 +1,10 @@
 """The block operators where they can go wrong: the order in which the e4m3 product's warps hand memory to one another, calls
 at the border of what the entry points take, and what they refuse.  Formulas, tolerances and helpers are test_block_ops'."""
+import ctypes
 import importlib
 import random
 import re
+import subprocess
 import threading
 import time
 from pathlib import Path
@@ -338,3 +340,143 @@ def test_calls_from_two_threads(native, quant):
     for thread in threads:
         thread.join()
     assert not wrong
+
+
+# ----------------------------------------------------------------------------------------- outputs that share memory
+OVERLAP_HARNESS = """
+#include "sq_overlap.h"
+static sq::View view(const long long* v) {
+  return sq::View(reinterpret_cast<const void*>(v[0]), v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
+}
+extern "C" int overlaps(const long long* a, const long long* b) { return sq::overlaps(view(a), view(b)); }
+extern "C" int overlaps_itself(const long long* a) { return sq::overlaps_itself(view(a)); }
+"""
+
+
+def test_overlap_of_views_against_their_bytes(pkg, tmp_path):
+    source, library = tmp_path / "harness.cpp", tmp_path / "harness.so"
+    source.write_text(OVERLAP_HARNESS)
+    csrc = ROOT / "fastwamjoint-quantization_b200" / "csrc"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", f"-I{csrc}", str(source), "-o", str(library)], check=True)
+    harness = ctypes.CDLL(str(library))
+    rng = random.Random(0)
+    pack = lambda v: (ctypes.c_longlong * 8)(*v)
+
+    def some_view():
+        nested = rng.random() < 0.5
+        counts = [rng.choice((1, 1, 2, 3, 5)) for _ in range(3)]
+        run = rng.choice((1, 2, 4, 8))
+        if nested:
+            inner = run + rng.choice((0, 0, 2))
+            middle = inner * counts[2] + rng.choice((0, 4))
+            strides = [middle * counts[1] + rng.choice((0, 16)), middle, inner]
+            if rng.random() < 0.3:
+                strides[0], strides[1], counts[0], counts[1] = strides[1], strides[0], counts[1], counts[0]
+        else:
+            strides = [rng.randrange(0, 24) for _ in range(3)]
+        return [rng.randrange(1, 160), run, counts[0], strides[0], counts[1], strides[1], counts[2], strides[2]]
+
+    def runs(v):
+        return [v[0] + i * v[3] + j * v[5] + k * v[7] for i in range(v[2]) for j in range(v[4]) for k in range(v[6])]
+
+    seen = {True: 0, False: 0}
+    for _ in range(4000):
+        a, b = some_view(), some_view()
+        if rng.random() < 0.4:  # neighbours in one packed row
+            b[1:] = a[1:]
+            b[0] = a[0] + rng.randrange(0, 40)
+        bytes_a = [x + i for x in runs(a) for i in range(a[1])]
+        bytes_b = {x + i for x in runs(b) for i in range(b[1])}
+        want = not bytes_b.isdisjoint(bytes_a)
+        seen[want] += 1
+        assert bool(harness.overlaps(pack(a), pack(b))) is want and bool(harness.overlaps(pack(b), pack(a))) is want
+        assert bool(harness.overlaps_itself(pack(a))) is (len(set(bytes_a)) < len(bytes_a))
+    assert min(seen.values()) > 500
+    for empty in ([0, 8, 1, 0, 1, 0, 1, 0], [64, 0, 1, 0, 1, 0, 1, 0], [64, 8, 0, 8, 1, 0, 1, 0]):
+        assert not harness.overlaps(pack(empty), pack([1, 200, 1, 0, 1, 0, 1, 0])) and not harness.overlaps_itself(pack(empty))
+
+
+def test_c_abi_refuses_overlap(pkg):
+    """Shared memory is found on the host; the pointers are never read (every call here is refused)."""
+    lib_mod = importlib.import_module(P + "_lib")
+    lib, refused = lib_mod.load_library(), lib_mod.ERR_OVERLAP
+    at = lambda kib: 1 << 20 | kib << 10  # tensors far apart
+    gemm = dict(codes=at(0), scales=at(64), rs=1, gs=4, w=at(128), ws=at(192), bias=at(256), out=at(320))
+
+    def product(**kw):
+        c = {**gemm, **kw}
+        return lib.sq_fp8_gemm(c["codes"], c["scales"], c["rs"], c["gs"], c["w"], c["ws"], c["bias"], c["out"], 0, 4, 16, 256, None)
+
+    for key in ("codes", "scales", "w", "ws", "bias"):
+        assert product(out=gemm[key]) == refused
+        assert product(**{key: gemm["out"] + 2 * 4 * 16 - 16}) == refused
+    quantize = lambda x, codes, scales, rs=1, gs=4: lib.sq_fp8_quantize(x, 0, 4, 256, 0, codes, scales, rs, gs, None)
+    assert quantize(at(0), at(0), at(64)) == refused and quantize(at(0), at(64), at(1)) == refused
+    assert quantize(at(0), at(64), at(64)) == refused and quantize(at(0), at(64), at(128), 1, 2) == refused
+    assert quantize(at(0), at(64), at(128), -1, 4) == lib_mod.ERR_SHAPE
+    linear = lambda x, w, ws, bias, out, work: lib.sq_fp8_linear(x, 0, 4, 256, 16, 0, w, ws, bias, out, work, 1 << 14, None)
+    apart = [at(64 * i) for i in range(6)]
+    for other in range(5):
+        assert linear(*[apart[other] if i == 5 else a for i, a in enumerate(apart)]) == refused
+    for other in (1, 2, 3):
+        assert linear(*[apart[other] if i == 4 else a for i, a in enumerate(apart)]) == refused
+
+    def norm(**kw):
+        base = dict(x=at(0), branch=at(64), h_out=at(128), z_out=at(192), rows=4, width=64, residual_scale=1.0, eps=1e-6,
+                    norm_kind=lib_mod.NORM_RMS)
+        return lib.sq_block_norm(lib_mod.ctypes.byref(lib_mod.BlockNorm(**{**base, **kw})), None)
+
+    row = lambda p: lib_mod.Param(p, 64, 1, 0)
+    for kw in (dict(h_out=at(0) + 128), dict(h_out=at(64) + 16), dict(z_out=at(128)), dict(z_out=at(0) + 16), dict(gate=row(at(128))),
+               dict(mod_shift=row(at(192))), dict(weight=lib_mod.Param(at(128) + 384)), dict(z_out=at(0), scales=at(256), scales_row_stride=1,
+                                                                                         scales_group_stride=4),
+               dict(scales=at(128), scales_row_stride=1, scales_group_stride=4), dict(scales=at(256))):
+        assert norm(**kw) == refused
+
+    def rotary(**kw):
+        strides = (lib_mod.c_int64 * 3)(512, 64, 32)
+        base = dict(q=at(0), k=at(64), q_out=at(128), k_out=at(192), positions=at(256), inv_freq=at(320), batch=1, length=8, heads=2, kv_heads=2,
+                    dim=32, axes=1, q_strides=strides, k_strides=strides, q_out_strides=strides, k_out_strides=strides, position_token_stride=1)
+        args = lib_mod.Rotary(**{**base, **{n: (lib_mod.c_int64 * 3)(*v) if isinstance(v, tuple) else v for n, v in kw.items()}})
+        args.sections[0] = 16
+        return lib.sq_rotary(lib_mod.ctypes.byref(args), None)
+
+    for kw in (dict(q_out=at(64)), dict(k_out=at(0)), dict(q_out=at(192)), dict(q_out=at(0) + 64), dict(q_out=at(0), q_out_strides=(512, 32, 256)),
+               dict(q_out_strides=(512, 32, 32)), dict(k_out_strides=(512, 32, 16)), dict(q_out=at(256)), dict(k_out=at(320)),
+               dict(norm=1, q_weight=at(128)), dict(norm=1, k_weight=at(128))):
+        assert rotary(**kw) == refused
+
+
+@gpu
+def test_outputs_that_share_memory_are_refused(native, quant, rope):
+    x, codes, scales, weight, weight_scales, bias = fp8_case(quant, 128, 128, 128, torch.bfloat16)
+    gemm = lambda out: native.fp8_gemm(codes, scales, weight, weight_scales, bias, out_dtype=torch.bfloat16, out=out)
+    room = torch.empty(128, 128, device="cuda", dtype=torch.bfloat16)
+    want = gemm(None)
+    assert torch.equal(gemm(room), want)
+    double = torch.zeros(2 * 128 * 128, device="cuda", dtype=torch.uint8)
+    codes_in = double[: 128 * 128].view(torch.float8_e4m3fn).view(128, 128)
+    with pytest.raises(ValueError, match="share no memory"):
+        native.fp8_gemm(codes_in, scales, weight, weight_scales, out_dtype=torch.bfloat16, out=double.view(torch.bfloat16).view(128, 128))
+    work = torch.empty(1 << 16, device="cuda", dtype=torch.uint8)
+    with pytest.raises(ValueError, match="share no memory"):
+        native.fp8_linear(x, weight, weight_scales, bias, workspace=work, out=work[: 2 * 128 * 128].view(torch.bfloat16).view(128, 128))
+    inside = x.clone()
+    want = native.fp8_linear(x, weight, weight_scales, bias)  # the quantizer has read x before the product writes
+    assert torch.equal(native.fp8_linear(inside, weight, weight_scales, bias, out=inside), want)
+
+    qkv = randn(2, 9, 6, 64, dtype=torch.bfloat16)
+    q, k = qkv[:, :, :4], qkv[:, :, 4:]
+    positions, freq = torch.arange(9, device="cuda", dtype=torch.int32)[:, None], rope.rotary_frequencies((32,), device="cuda")
+    turn = lambda q, k, out=None: native.rotary(q, k, positions, freq, sections=(32,), out=out)
+    spare = torch.empty(2, 9, 4, 64, device="cuda", dtype=torch.bfloat16)
+    late = torch.empty(2, 10, 6, 64, device="cuda", dtype=torch.bfloat16)
+    late[:, :9] = qkv
+    for inputs, out in (((q, k), (qkv[:, :, 1:5], None)), ((q, k), (spare, spare[:, :, :2])), ((q, k), (None, q[:, :, :2])),
+                        ((late[:, :9, :4], None), (late[:, 1:, :4], None)),
+                        ((q, None), (spare.flatten()[: 2 * 9 * 4 * 64].as_strided((2, 9, 4, 64), (2304, 64, 64, 1)), None))):
+        with pytest.raises(ValueError, match="share no memory"):
+            turn(*inputs, out=out)
+    want = turn(q, k)
+    turn(q, k, out=(q, k))  # neighbours in one packed tensor, each its own input
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
