@@ -572,28 +572,39 @@ _ROTARY_LAYOUTS = {"interleaved": _lib.ROTARY_INTERLEAVED, "half": _lib.ROTARY_H
 _ROTARY_NORMS = {None: _lib.ROTARY_NORM_NONE, "head": _lib.ROTARY_NORM_HEAD, "token": _lib.ROTARY_NORM_TOKEN}
 
 
+def _heads_strides(t: torch.Tensor):
+    """Batch, token and head strides of [batch, tokens, heads, dim]; an axis of one index has none of its own and gets one
+    on the vector grid."""
+    (b, s, h, _), (batch, tokens, heads, dim) = t.stride(), t.shape
+    if heads == 1:
+        h = dim
+    if batch == 1 and b % 8:
+        b = 0
+    if tokens == 1 and s % 8:
+        s = b
+    return b, s, h
+
+
 def _heads_input(t: torch.Tensor):
     """(tensor, pointer, batch / token / head strides) with vectors the kernel can read in place, or a copy that has them."""
-    b, s, h, d = t.stride()
-    pointer = t.data_ptr()
-    if d != 1 or (b | s | h) % 8 or pointer % 16:
+    b, s, h = _heads_strides(t)
+    if t.stride(3) != 1 or (b | s | h) % 8 or t.data_ptr() % 16:
         t = _vectors(t)
-        b, s, h, d = t.stride()
-        pointer = t.data_ptr()
-    return t, pointer, (b, s, h)
+        b, s, h = _heads_strides(t)
+    return t, t.data_ptr(), (b, s, h)
 
 
 def _heads_output(out, like, shape, dtype, device, name: str):
     if out is None:
         out = like.new_empty(shape)
         return out, out.data_ptr(), (shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3])
-    strides = out.stride()
-    fits = (out.shape == shape and out.dtype is dtype and out.device == device and strides[3] == 1 and out.data_ptr() % 16 == 0
-            and all(s % 8 == 0 and (s > 0 or n == 1) for s, n in zip(strides[:3], shape)))
+    fits = out.shape == shape and out.dtype is dtype and out.device == device and out.stride(3) == 1 and out.data_ptr() % 16 == 0
+    strides = _heads_strides(out) if fits else None
+    fits = fits and all(s % 8 == 0 and (s > 0 or n == 1) for s, n in zip(strides, shape))
     if not fits:
         raise ValueError(f"out for {name} must match it, with a contiguous last axis, strides that are multiples of 8 "
                          "elements and 16-byte alignment.")
-    return out, out.data_ptr(), strides[:3]
+    return out, out.data_ptr(), strides
 
 
 def _rotary_weight(t, kept: list, count: int, dim: int, norm, dtype, device, name: str):

@@ -480,3 +480,22 @@ def test_outputs_that_share_memory_are_refused(native, quant, rope):
     want = turn(q, k)
     turn(q, k, out=(q, k))  # neighbours in one packed tensor, each its own input
     assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
+# ---------------------------------------------------------------------------------------------------------- rotary
+@gpu
+@pytest.mark.parametrize("shape", [(1, 1, 1, 64), (1, 1, 3, 64), (2, 1, 1, 64), (1, 5, 1, 64), (3, 1, 2, 64)])
+def test_rotary_strides_of_axes_with_one_index(native, rope, shape):
+    """An axis of one index may have any stride: a single token or head cut out of a wider tensor."""
+    x = randn(*shape, dtype=torch.bfloat16)
+    batch, tokens, heads, dim = shape
+    positions, freq = torch.arange(3, 3 + tokens, device="cuda", dtype=torch.int32)[:, None], rope.rotary_frequencies((32,), device="cuda")
+    turn = lambda t, out=None: native.rotary(t, None, positions, freq, sections=(32,), out=out)[0]
+    want = turn(x)
+    strides = [67 if n == 1 else s for n, s in zip(shape[:3], x.stride())]
+    odd = torch.zeros(batch * tokens * heads * dim, device="cuda", dtype=torch.bfloat16).as_strided(shape, (*strides, 1))
+    odd.copy_(x)
+    assert torch.equal(turn(odd), want)
+    room = torch.zeros_like(x).as_strided(shape, (*strides, 1))
+    assert turn(x, (room, None)) is room and torch.equal(room, want)
+    assert torch.equal(turn(odd, (odd, None)), want) and torch.equal(odd, want)
