@@ -499,3 +499,23 @@ def test_rotary_strides_of_axes_with_one_index(native, rope, shape):
     room = torch.zeros_like(x).as_strided(shape, (*strides, 1))
     assert turn(x, (room, None)) is room and torch.equal(room, want)
     assert torch.equal(turn(odd, (odd, None)), want) and torch.equal(odd, want)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("dim,pairs", [(16, 3), (64, 5), (64, 8), (72, 14), (128, 62), (128, 63)])
+def test_rotary_passes_the_rest_of_a_head_through(native, rope, dim, pairs, layout, dtype):
+    """Elements past the turned pairs come out bit for bit, infinities and negative zeros too, and disturb nothing."""
+    x = randn(2, 7, 3, dim, dtype=dtype)
+    rest = x[..., 2 * pairs:]
+    rest[..., 0::3], rest[..., 1::4], rest[0, 0, 0, -1] = float("inf"), -0.0, float("nan")
+    positions, freq = torch.arange(1, 8, device="cuda", dtype=torch.int32)[:, None], rope.rotary_frequencies((pairs,), device="cuda")
+    got = native.rotary(x, None, positions, freq, sections=(pairs,), layout=layout)[0]
+    nan = rest.isnan()
+    assert torch.equal(got[..., 2 * pairs:].isnan(), nan)
+    assert torch.equal(got[..., 2 * pairs:].view(torch.int16)[~nan], rest.view(torch.int16)[~nan])
+    alone = x.clone()
+    alone[..., 2 * pairs:] = 0
+    alone = native.rotary(alone, None, positions, freq, sections=(pairs,), layout=layout)[0]
+    assert torch.equal(got[..., :2 * pairs], alone[..., :2 * pairs]) and alone.isfinite().all()
