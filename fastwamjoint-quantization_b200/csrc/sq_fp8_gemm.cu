@@ -288,6 +288,7 @@ __global__ void __launch_bounds__(128 + 32 * few_drain_warps(TOK), 1)
         if (lane == 0) report_timeout(p.status, abort_flag, 9204);
         return false;
       }
+      __syncwarp();  // lanes may leave the wait one by one; the loads below are the whole warp's
       tc_fence_after_sync();
       uint32_t d[kCols];
       tmem_ld_chunk(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * TOK + share * kCols, d);
@@ -666,9 +667,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         tc_fence_after_sync();
         const uint32_t from = lanes + acc * 128;
         tmem_ld_32x32b_x32(from, d[0]);
-        if ((run & 3u) == 0 && !mbar_wait_bounded(bar_factor + ((run << 1) & 8u), (run >> 3) & 1u, abort_flag, kWaitLimitNs)) {
-          if (lane == 0) report_timeout(p.status, abort_flag, 9216);
-          goto out;
+        if ((run & 3u) == 0) {
+          if (!mbar_wait_bounded(bar_factor + ((run << 1) & 8u), (run >> 3) & 1u, abort_flag, kWaitLimitNs)) {
+            if (lane == 0) report_timeout(p.status, abort_flag, 9216);
+            goto out;
+          }
+          __syncwarp();  // the wait for the loads below is the whole warp's
         }
         asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(my_factors + (run & 7u) * kFactorBytes) : "memory");
 #pragma unroll
