@@ -321,7 +321,7 @@ int launch_fp8_quantize(const void* x, int x_dtype, int64_t rows, int64_t K, int
   const int64_t per_row = (K + 127) / 128;
   if (rows > (int64_t{1} << 30) / per_row) return SQ_ERR_SHAPE;
   if (scales_row < 0 || scales_group < 0) return SQ_ERR_SHAPE;
-  const View from(x, rows * K * 2), to(codes, rows * K), scale_view(scales, 4, rows, scales_row * 4, per_row, scales_group * 4);
+  const View from(x, rows * K * 2), to(codes, rows * K), scale_view(scales, 4, per_row, scales_group * 4, rows, scales_row * 4);
   if (clashes(to, {from, scale_view}) || clashes(scale_view, {from})) return SQ_ERR_OVERLAP;
   const uint32_t runs = static_cast<uint32_t>(rows * per_row);
   const Divisor by = divisor(per_row);
@@ -342,23 +342,26 @@ int launch_fp8_quantize(const void* x, int x_dtype, int64_t rows, int64_t K, int
 // h and z may take the place of x or branch, row by row; else what is written shares memory with nothing.
 static int norm_overlap(const SqBlockNorm& b) {
   const int64_t bytes = b.rows * b.width;
-  const View x(b.x, 2 * bytes), branch(b.branch, 2 * bytes);
-  const View h(b.branch != nullptr ? b.h_out : nullptr, 2 * bytes);
-  const View z(b.norm_kind != SQ_NORM_NONE ? b.z_out : nullptr, b.scales != nullptr ? bytes : 2 * bytes);
-  const View scales(b.scales, 4, b.rows, 4 * b.scales_row_stride, (b.width + 127) / 128, 4 * b.scales_group_stride);
-  auto channels = [&](const SqParam& q) { return View(q.data, b.width * (q.is_fp32 ? 4 : 2)); };
-  auto table = [&](const SqParam& q) {
-    const int64_t size = q.is_fp32 ? 4 : 2, groups = q.data == nullptr || q.span <= 0 ? 1 : (b.rows + q.span - 1) / q.span;
-    return View(q.data, b.width * size, groups, q.row_stride * size);
-  };
-  for (const View& out : {h, z, scales}) {
-    if (clashes(out, {channels(b.post_weight), channels(b.post_bias), channels(b.weight), channels(b.bias), table(b.gate),
-                      table(b.mod_scale), table(b.mod_shift)}))
-      return SQ_ERR_OVERLAP;
-    for (const View& in : {x, branch})
-      if (!same_view(out, in) && overlaps(out, in)) return SQ_ERR_OVERLAP;
+  const View in[2] = {View(b.x, 2 * bytes), View(b.branch, 2 * bytes)};
+  const View out[3] = {View(b.branch != nullptr ? b.h_out : nullptr, 2 * bytes),
+                       View(b.norm_kind != SQ_NORM_NONE ? b.z_out : nullptr, b.scales != nullptr ? bytes : 2 * bytes),
+                       View(b.scales, 4, (b.width + 127) / 128, 4 * b.scales_group_stride, b.rows, 4 * b.scales_row_stride)};
+  const SqParam* params[7] = {&b.gate, &b.mod_scale, &b.mod_shift, &b.post_weight, &b.post_bias, &b.weight, &b.bias};
+  for (int i = 0; i < 7; ++i) {
+    const SqParam& q = *params[i];
+    if (q.data == nullptr) continue;
+    const int64_t size = q.is_fp32 ? 4 : 2, rows = i < 3 && q.span < b.rows ? (b.rows + q.span - 1) / q.span : 1;
+    const View read(q.data, b.width * size, rows, i < 3 ? q.row_stride * size : 0);
+    if (overlaps(out[0], read) || overlaps(out[1], read) || overlaps(out[2], read)) return SQ_ERR_OVERLAP;
   }
-  return overlaps(h, z) || overlaps(h, scales) || overlaps(z, scales) ? SQ_ERR_OVERLAP : SQ_OK;
+  for (int i = 0; i < 3; ++i) {
+    if (overlaps_itself(out[i])) return SQ_ERR_OVERLAP;
+    for (int j = 0; j < 2; ++j)
+      if (overlaps(out[i], in[j]) && !same_view(out[i], in[j])) return SQ_ERR_OVERLAP;
+    for (int j = 0; j < i; ++j)
+      if (overlaps(out[i], out[j])) return SQ_ERR_OVERLAP;
+  }
+  return SQ_OK;
 }
 
 int launch_block_norm(const SqBlockNorm& b, cudaStream_t stream) {

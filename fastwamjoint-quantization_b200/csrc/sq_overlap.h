@@ -81,6 +81,14 @@ inline bool overlaps(const View& a, const View& b) {
 inline bool overlaps_itself(const View& a) {
   using overlap::Wide;
   if (a.empty) return false;
+  Wide inside = a.run;  // axes that contain one another in order, as most do: nothing to look for
+  bool nested = true;
+  for (int i = 2; i >= 0; --i) {
+    if (a.count[i] == 1) continue;
+    nested = nested && a.stride[i] >= inside;
+    inside += Wide{a.stride[i]} * (a.count[i] - 1);
+  }
+  if (nested) return false;
   for (int lead = 0; lead < 3; ++lead) {  // indices that differ first on axis `lead`, there by one or more
     const Wide most = Wide{a.count[lead]} - 1;
     if (most <= 0) continue;

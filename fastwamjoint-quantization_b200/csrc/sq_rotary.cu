@@ -455,17 +455,20 @@ static int rotary_overlap(const SqRotary& r, int pairs) {
   auto heads = [&](const void* at, int32_t count, const int64_t (&s)[3]) {
     return View(at, 2 * r.dim, r.batch, 2 * s[0], r.length, 2 * s[1], count, 2 * s[2]);
   };
-  const View q = heads(r.q, r.heads, r.q_strides), q_out = heads(r.q_out, r.heads, r.q_out_strides);
-  const View k = heads(r.k, r.kv_heads, r.k_strides), k_out = heads(r.k_out, r.kv_heads, r.k_out_strides);
-  const int token = r.norm == SQ_ROTARY_NORM_TOKEN, size = r.position_type == SQ_POS_INT64 ? 8 : 4;
-  const View q_weight(r.q_weight, (r.q_weight_fp32 ? 4 : 2) * r.dim * (token ? r.heads : 1));
-  const View k_weight(r.k_weight, (r.k_weight_fp32 ? 4 : 2) * r.dim * (token ? r.kv_heads : 1));
-  const View positions(r.positions, size * r.axes, r.batch, size * r.position_batch_stride, r.length, size * r.position_token_stride);
-  const View inv_freq(r.inv_freq, 8 * pairs);
-  for (const View& out : {q_out, k_out})
-    if (clashes(out, {q_weight, k_weight, positions, inv_freq})) return SQ_ERR_OVERLAP;
-  if ((!same_view(q_out, q) && overlaps(q_out, q)) || (!same_view(k_out, k) && overlaps(k_out, k))) return SQ_ERR_OVERLAP;
-  return overlaps(q_out, k) || overlaps(k_out, q) || overlaps(q_out, k_out) ? SQ_ERR_OVERLAP : SQ_OK;
+  const int weights = r.norm == SQ_ROTARY_NORM_TOKEN ? r.dim : 0, size = r.position_type == SQ_POS_INT64 ? 8 : 4;
+  const View out[2] = {heads(r.q_out, r.heads, r.q_out_strides), heads(r.k_out, r.kv_heads, r.k_out_strides)};
+  const View read[6] = {heads(r.q, r.heads, r.q_strides),
+                        heads(r.k, r.kv_heads, r.k_strides),
+                        View(r.q_weight, (r.q_weight_fp32 ? 4 : 2) * (weights > 0 ? weights * r.heads : r.dim)),
+                        View(r.k_weight, (r.k_weight_fp32 ? 4 : 2) * (weights > 0 ? weights * r.kv_heads : r.dim)),
+                        View(r.positions, size * r.axes, r.batch, size * r.position_batch_stride, r.length, size * r.position_token_stride),
+                        View(r.inv_freq, 8 * pairs)};
+  for (int i = 0; i < 2; ++i) {
+    if (overlaps_itself(out[i])) return SQ_ERR_OVERLAP;
+    for (int j = 0; j < 6; ++j)
+      if (overlaps(out[i], read[j]) && !(i == j && same_view(out[i], read[j]))) return SQ_ERR_OVERLAP;
+  }
+  return overlaps(out[0], out[1]) ? SQ_ERR_OVERLAP : SQ_OK;
 }
 
 int launch_rotary(const SqRotary& r, cudaStream_t stream) {
