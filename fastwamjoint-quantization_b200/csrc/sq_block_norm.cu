@@ -107,18 +107,21 @@ __device__ __forceinline__ void standardise(float (&v)[VPT][8], const bool (&on)
     }
   }
   float squares = row_sum(local_squares(v));
-  if (!(squares < __int_as_float(0x7F800000))) {
-    // the squares of bf16 values beyond 2^59 or so overflow: the row over again, 2^70 times smaller (eps is nothing next
-    // to such a row).  The sum is the same in every thread of the row, so all of them come here or none.
+  float mean_square = fmaf(squares, inv_width, eps);
+  if (!(mean_square > 1e-30f && squares < __int_as_float(0x7F800000))) {
+    // the squares of bf16 values beyond 2^59 or so overflow, and those of tiny ones vanish where eps does not cover them: the
+    // row over again, 2^70 times smaller or larger.  The sum is the same in every thread of the row, so all of them come here
+    // or none.
+    const float by = squares < 1.0f ? 1180591620717411303424.0f : 8.470329472543003e-22f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] *= 8.470329472543003e-22f;
+      for (int e = 0; e < 8; ++e) v[i][e] *= by;
     }
     squares = row_sum(local_squares(v));
-    eps = 0.0f;
+    mean_square = fmaf(squares, inv_width, eps * by * by);
   }
-  const float r = __frsqrt_rn(fmaf(squares, inv_width, eps));
+  const float r = __frsqrt_rn(mean_square);
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
 #pragma unroll

@@ -634,9 +634,9 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     int64 or float32, any value, however far or negative: angles are reduced in 64 bits (the rotation by
     ``-positions`` undoes it).  ``layout``: pairs are neighbours ("interleaved") or half the rotated length apart
     ("half"); elements past 2 * pairs pass through.  ``norm``: RMS of each head ("head", weights [dim]) or over all
-    heads of a token ("token", weights [heads * dim]), statistics in fp32 (values up to 2^59).  ``out`` is a pair (q, k) of
-    tensors to write, strided as a cache or a transposed view may be; they may be the inputs themselves, and share
-    no memory with an input, each other or themselves otherwise (refused)."""
+    heads of a token ("token", weights [heads * dim]), statistics in fp32 (values up to 2^56, and from 2^-56 where eps is
+    zero).  ``out`` is a pair (q, k) of tensors to write, strided as a cache or a transposed view may be; they may be the
+    inputs themselves, and share no memory with an input, each other or themselves otherwise (refused)."""
     if out is None and (pair := _binding.rotary(q, k, positions, inv_freq, sections, layout, norm, q_weight, k_weight, eps)) is not None:
         return pair
     if not q.is_cuda:

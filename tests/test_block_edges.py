@@ -12,7 +12,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from test_block_ops import DTYPES, P, fp8_case, fp8_product, fp8_slack, gpu, half_step, no_device_timeouts, randn, within  # noqa: F401
+from test_block_ops import DTYPES, P, check_block_norm, fp8_case, fp8_product, fp8_slack, gpu, half_step, no_device_timeouts, randn, within  # noqa: F401
 
 ROOT = Path(__file__).resolve().parents[1]
 
@@ -519,3 +519,18 @@ def test_rotary_passes_the_rest_of_a_head_through(native, rope, dim, pairs, layo
     alone[..., 2 * pairs:] = 0
     alone = native.rotary(alone, None, positions, freq, sections=(pairs,), layout=layout)[0]
     assert torch.equal(got[..., :2 * pairs], alone[..., :2 * pairs]) and alone.isfinite().all()
+
+
+# -------------------------------------------------------------------------------------------------------- block norms
+@gpu
+@pytest.mark.parametrize("eps", [0.0, 1e-35, 1e-12])
+@pytest.mark.parametrize("width", [64, 1000, 2048, 4096, 6144, 14336])
+def test_block_norm_of_tiny_and_huge_rows(native, width, eps):
+    """Rows whose squares leave the range of fp32 on either side, with an eps that does not cover the small ones."""
+    x = randn(7, width) * torch.tensor([1e-30, 1e-25, 1e-19, 1e-15, 1.0, 1e19, 1e30], device="cuda")[:, None]
+    x, branch = x.bfloat16(), x.flip(1).bfloat16()
+    check_block_norm(native, x, norm="rms", eps=eps)
+    check_block_norm(native, x, norm="layer", eps=eps)
+    check_block_norm(native, torch.zeros_like(x), branch, post_norm="rms", norm="layer", eps=eps)
+    _, z = native.block_norm(torch.zeros_like(x), norm="rms", eps=max(eps, 1e-35))
+    assert not z.any()
