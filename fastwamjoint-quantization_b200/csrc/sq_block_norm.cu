@@ -43,7 +43,7 @@ struct NormArgs {
 // Sum over the threads of a block, the same value in each of them and the same order in every run.  Two buffers in turn:
 // one barrier per sum (a buffer is written again two sums later, past the barrier of the sum between).  Up to eight warps'
 // parts are added by every thread: two wide reads of the same address and a short tree take less time than shuffles
-// (measured with the divisions below: 32768 x 4096 at 221 us, 231 before); sixteen and more parts cost registers that spill.
+// (measured with the divisions below: 32768 x 4096 at 221 us where it took 231); sixteen and more parts cost registers that spill.
 template <int kWarps>
 struct RowSum {
   static constexpr int kParts = kWarps < 4 ? 4 : kWarps;
@@ -241,12 +241,15 @@ int launch_shape(const NormArgs& a, cudaStream_t stream) {
   return err == cudaSuccess ? SQ_OK : static_cast<int>(err);
 }
 
-// One vector per thread up to 1024 elements, else two; registers are held to what lets 64 / 48 warps live on an SM (the more
-// rows under way, the better HBM is used, until values spill).  Measured at 32768 x 4096 fp16 with fp32 modulation: two vectors
-// and 32 / 40 / 48 / 64 warps 259 / 233 / 236 / 289 us, one vector and 64 warps 247 (48 warps with 32-byte parameter loads: 227); at 4096 x 5120 with a modulation row per
-// token 72 / 72 / 61 / 62 us; at 32 x 1024 one vector 2.4 us, two 3.2.  Beyond 8192 a block of two vectors per thread fills an
-// SM, and two blocks of four vectors overlap one's loads with the other's sums: 232 us instead of 257 at 8192 x 12288, 259
-// instead of 275 at 8192 x 16384, but 8.2 instead of 5.7 where 64 rows leave SMs idle.
+// One vector per thread up to 1024 elements, else two; registers are held to what lets 64 / 48 warps live on an SM: the more
+// rows under way, the better HBM is used.  The forms with a branch pay for it with spills (ptxas: 16 to 64 bytes of stores a
+// thread beyond 1024 elements), and are faster all the same.  Measured at 32768 x 4096 fp16 with fp32 modulation, before its
+// parameters were read 32 bytes at a time: two vectors and 32 / 40 / 48 / 64 warps 259 / 233 / 236 / 289 us, one vector and 64
+// warps 247 (225 now); at 4096 x 5120 with a modulation row per token 72 / 72 / 61 / 62 us; at 32 x 1024 one vector 2.4 us,
+// two 3.2.  Beyond 8192 a block of two vectors per thread fills an SM, and two blocks of four vectors overlap one's loads with
+// the other's sums.  With two rows for each of 148 SMs or more that is faster on the whole; two RMS norms, two vectors against
+// four: 12288 wide 9.6 / 9.8 us at 296 rows, 13.4 / 15.9 at 444, 18.4 / 18.0 at 592, 228 / 193 at 8192; 16384 wide 11.6 / 10.8,
+// 17.5 / 19.7, 25 / 23.8, 280 / 245.  Where 64 rows leave SMs idle it is 8.2 instead of 5.7.
 template <typename T>
 int launch_typed(const NormArgs& a, cudaStream_t stream) {
   if (a.width <= 512) return launch_shape<T, 1, 64, 32>(a, stream);

@@ -294,7 +294,7 @@ int sq_linear_noalloc(const void* x, int x_dtype, int64_t rows, int64_t K, int64
 /* Activations to e4m3: x [rows, K] bf16 / fp16 (x_dtype) -> codes [rows, K] and one fp32 scale per row and run of 128 k
  * (the last run may be shorter): scale = max(amax / 448, 1e-8), code = e4m3(x * (1 / scale)), round to nearest even,
  * saturating.  A run with a NaN or an infinity gets a scale of that kind and its row of a product comes out NaN.
- * scales[row, run] lies at row * scales_row_stride + run * scales_group_stride.  input_activation: SQ_ACT_FN_GELU applies
+ * scales[row, run] lies at row * scales_row_stride + run * scales_group_stride (not negative).  input_activation: SQ_ACT_FN_GELU applies
  * the erf GELU in fp32 first.  K % 16 == 0, K <= 131072; x and codes 16-byte aligned. */
 int sq_fp8_quantize(const void* x, int x_dtype, int64_t rows, int64_t K, int input_activation, void* codes, float* scales,
                     int64_t scales_row_stride, int64_t scales_group_stride, void* stream);
