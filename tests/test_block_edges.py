@@ -45,7 +45,8 @@ class Barrier:
 
 def pair_kernel(stages, parts, runs, rng, free_by_readers):
     """One pair of thread blocks of ``sq_fp8_pair_kernel`` at the grain of its barriers, its warps stepped in random order:
-    what a drain warp read in place of its run's factors, or None.  ``stages``: of the operand ring; ``parts``: products a
+    the first operand, accumulator or factor that a warp found in place of its own run's, every warp
+    waiting, or None.  ``stages``: of the operand ring; ``parts``: products a
     run (1: 128 channels, 2: 256).  ``free_by_readers``: a place for factors is free when its readers say so; otherwise
     when the MMAs of a later run are done."""
     blocks, depth, drains = (0, 1), 4 // parts, 2
@@ -56,11 +57,15 @@ def pair_kernel(stages, parts, runs, rng, free_by_readers):
     ready = [[Barrier(1) for _ in range(2)] for _ in blocks]
     free = [[Barrier(drains) for _ in range(2)] for _ in blocks]
     slots = [[None] * 8 for _ in blocks]
+    operands = [[None] * stages for _ in blocks]
+    accumulators = [[None] * 4 for _ in blocks]
     wrong = []
 
     def producer(block):
         for run in range(runs):
             yield lambda: empty[block][run % stages].passed((run // stages & 1) ^ 1)
+            operands[block][run % stages] = run
+            yield lambda: True
             full[run % stages].arrive()
 
     def issuer(mine):
@@ -68,8 +73,13 @@ def pair_kernel(stages, parts, runs, rng, free_by_readers):
             run, acc = product // parts, product % 4
             yield lambda: full[run % stages].passed(run // stages & 1)
             yield lambda: acc_empty[acc].passed((product // 4 & 1) ^ 1)
+            for block in blocks:
+                accumulators[block][acc] = None
             yield lambda: True  # the MMAs end some time after
             for block in blocks:
+                if operands[block][run % stages] != run:
+                    wrong.append(("operand", run, operands[block][run % stages]))
+                accumulators[block][acc] = product
                 acc_full[block][acc].arrive()
                 empty[block][run % stages].arrive()
 
@@ -93,8 +103,10 @@ def pair_kernel(stages, parts, runs, rng, free_by_readers):
             yield lambda: acc_full[block][acc].passed(turn & 1)
             if run % 4 == 0:
                 yield lambda: ready[block][run >> 2 & 1].passed(run >> 3 & 1)
+            if accumulators[block][acc] != (run if parts == 1 else 2 * run + share):
+                wrong.append(("accumulator", run, accumulators[block][acc]))
             if slots[block][run & 7] != run:
-                wrong.append((run, slots[block][run & 7]))
+                wrong.append(("factor", run, slots[block][run & 7]))
             acc_empty[acc].arrive()
             yield lambda: True
             if run % 4 == 3:
@@ -106,7 +118,8 @@ def pair_kernel(stages, parts, runs, rng, free_by_readers):
     pace = {warp: rng.choice((1, 1, 1, 40)) for warp in warps}
     while any(wait is not None for wait in waiting.values()):
         able = [warp for warp, wait in waiting.items() if wait is not None and wait()]
-        assert able, "every warp waits"
+        if not able:
+            return "every warp waits"
         warp = rng.choices(able, [1 / pace[warp] for warp in able])[0]
         waiting[warp] = next(warp, None)
         if wrong:
@@ -316,7 +329,7 @@ def test_other_threads_run_while_a_call_waits(native):
     torch.cuda.synchronize()
     assert waited > 0.2, "the launches did not wait for the device"
     longest = max(b - a for a, b in zip(ticks, ticks[1:]))
-    assert longest < waited / 4
+    assert longest < waited / 2
 
 
 @gpu
